@@ -1,0 +1,393 @@
+"""Scoring of given tokens (`ops.score`) against plain formulas in 64 bits.
+
+Bounds.  With u = (x - max x) / T and z = sum exp u, an fp32 result carries: the roundings of u (difference, factor, product)
+and of the last sum and product, 6 x 2^-24 of |u| + log z; of an exponential 2^-22 and what its argument is off by; of a sum
+at most one rounding an addition, and no accumulator takes more than a 128th of a row.  So the log-probability is off by at
+most 2^-24 (V / 128 + 64) (1 + |u| + log V), and the entropy, whose terms are probabilities times |u|, by twice that.
+"""
+import math
+
+import pytest
+import torch
+
+from xllm_b200.ops import score
+
+STEP = 2.0 ** -24
+
+
+def exact(x, ids, n_top=0, temperature=None):
+    """(logprob, entropy, alternatives, their log-probabilities, |u| of the given tokens) in 64 bits, a row at a time."""
+    lps, ents, tops, top_lps, far = [], [], [], [], []
+    V = x.shape[1]
+    for r in range(x.shape[0]):
+        row, i = x[r].double().cpu(), int(ids[r])
+        T = 1.0 if temperature is None or not float(temperature[r]) > 0 else float(temperature[r])
+        bad = bool(torch.isnan(row).any()) or bool((row == math.inf).any())
+        live = row[~torch.isnan(row)]
+        none = not bad and bool((row == -math.inf).all())
+        m = 0.0 if none else (float(live.max()) if len(live) else 0.0)
+        u = (row - m) / T
+        z = torch.exp(u).sum()
+        p = torch.exp(u) / z
+        lp = torch.log(torch.exp(u) / z) if none or bad else u - torch.log(z)
+        ents.append(math.nan if bad else 0.0 if none else float(torch.log(z) - torch.where(p > 0, p * u, 0.0).sum()))
+        lps.append(0.0 if i < 0 else -math.inf if i >= V or none else math.nan if bad else float(lp[i]))
+        far.append(0.0 if not 0 <= i < V or none or bad or u[i] == -math.inf else abs(float(u[i])))
+        order = []
+        if n_top:
+            sized, by = torch.sort(torch.where(torch.isnan(row), -math.inf, row), descending=True, stable=True)
+            order = by[:n_top][sized[:n_top] > -math.inf].tolist()
+        tops.append(order + [-1] * (n_top - len(order)))
+        top_lps.append([math.nan if bad else float(lp[j]) for j in order] + [-math.inf] * (n_top - len(order)))
+    d = lambda v: torch.tensor(v, dtype=torch.float64)
+    return d(lps), d(ents), torch.tensor(tops).view(len(tops), -1), d(top_lps).view(len(tops), -1), d(far)
+
+
+def near(got, want, bound, what):
+    got = got.double().cpu()
+    same = torch.isnan(got) & torch.isnan(want) | (got == want)
+    off = torch.where(same, 0.0, (got - want).abs())
+    assert bool((off <= bound).all()), f"{what}: {off.max()} off, {got.flatten()[off.argmax()]} for {want.flatten()[off.argmax()]}"
+
+
+def compare(got, x, ids, n_top=0, temperature=None):
+    lp, ent, top, top_lp, far = exact(x, ids, n_top, temperature)
+    V = x.shape[1]
+    unit = STEP * (V / 128 + 64)
+    near(got[0], lp, unit * (1 + far + math.log(V)), "logprob")
+    near(got[1], ent, 2 * unit * (1 + math.log(V)), "entropy")
+    if n_top == 0:
+        assert len(got) == 2 or got[2] is None and got[3] is None
+        return
+    assert got[2].dtype == torch.int32 and torch.equal(got[2].long().cpu(), top.long()), "alternatives"
+    near(got[3], top_lp, unit * (1 + math.log(V) + torch.where(top_lp > -math.inf, top_lp.abs(), 0.0)), "alternatives' logprob")
+
+
+def rows(n, V, dtype, seed, device, pad=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(n, V + pad, generator=g) * spread).to(dtype).to(device)
+    ids = torch.randint(0, V, (n,), generator=g).to(device)
+    t = (torch.rand(n, generator=g) * 1.5 + 0.2).to(device)
+    return x[:, pad:], ids, t
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,V,n_top,pad", [(1, 1, 1, 0), (3, 2, 2, 0), (5, 7, 3, 1), (2, 255, 20, 0), (4, 1000, 5, 3), (7, 4099, 1, 5),
+                                           (2, 9001, 128, 1), (33, 2048, 0, 0), (1, 20011, 64, 7)])
+def test_rows(device, dtype, n, V, n_top, pad):
+    x, ids, t = rows(n, V, dtype, n * V, device, pad)
+    compare(score.token_logprobs(x, ids, n_top), x, ids, n_top)
+    compare(score.token_logprobs(x, ids, n_top, temperature=t), x, ids, n_top, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 2, 9, 40, 150, 700, 2500])
+def test_row_counts(n):
+    """Few rows are split over several blocks, many are not: the same results either way."""
+    x, ids, t = rows(n, 6007, torch.bfloat16, 3, "cuda", 3)
+    got = score.token_logprobs(x, ids, 6, temperature=t)
+    pick = sorted({0, n // 2, n - 1})
+    at = torch.tensor(pick, device="cuda")
+    compare(tuple(g[at] for g in got), x[at], ids[at], 6, t[at])
+    one = score.token_logprobs(x[:1], ids[:1], 6, temperature=t[:1])
+    assert torch.equal(one[2], got[2][:1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [1, 300])
+def test_whole_vocabulary(dtype, n):
+    x, ids, t = rows(n, 151936, dtype, 11, "cuda")
+    got = score.token_logprobs(x, ids, 20, temperature=t)
+    at = torch.tensor(sorted({0, n // 3, n - 1}), device="cuda")
+    compare(tuple(g[at] for g in got), x[at], ids[at], 20, t[at])
+
+
+def edge_rows(V, dtype):
+    """Rows where a softmax goes wrong, and the token asked for in each."""
+    low, inf = torch.finfo(dtype).min, math.inf
+    g = torch.Generator().manual_seed(5)
+    base = lambda: torch.randn(V, generator=g) * 2
+    out = []
+
+    def add(row, i):
+        out.append((row.to(dtype), i))
+    add(torch.full((V,), -inf), 1)                                    # a mask that leaves nothing
+    r = torch.full((V,), -inf); r[V - 1] = 3.0; add(r, V - 1)         # ... and one token
+    add(r.clone(), 0)                                                 # a masked token is asked for
+    r = base(); r[: V // 2] = low; add(r, V - 1)                      # masks of the type's lowest value
+    add(r.clone(), 0)
+    add(torch.full((V,), low), V // 2)                                # nothing but those
+    add(torch.zeros(V), V - 1)                                        # all tokens alike
+    r = base(); r[V // 3] = math.nan; add(r, 0)
+    r = base(); r[V // 3] = inf; add(r, V // 3)
+    r = torch.full((V,), -inf); r[2] = math.nan; add(r, 2)
+    r = base(); r[V // 2] = 90.0; add(r, V // 2)                      # certain
+    add(r.clone(), 0)
+    add(base(), -1)                                                   # nothing asked
+    add(base(), V)                                                    # beyond the vocabulary
+    add(base(), -(1 << 40))
+    add(base() * 1e-30, 3)
+    r = torch.zeros(V); r[1::2] = -0.0; add(r, 1)                     # zeros of both signs tie
+    return torch.stack([r for r, _ in out]), torch.tensor([i for _, i in out])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,n_top", [(37, 5), (1500, 20), (6001, 3)])
+@pytest.mark.parametrize("each", [True, False])
+def test_edges(device, dtype, V, n_top, each):
+    x, ids = edge_rows(V, dtype)
+    x, ids = x.to(device), ids.to(device)
+    if each:
+        for r in range(x.shape[0]):
+            compare(score.token_logprobs(x[r:r + 1], ids[r:r + 1], n_top), x[r:r + 1], ids[r:r + 1], n_top)
+    else:
+        compare(score.token_logprobs(x.repeat(40, 1), ids.repeat(40), n_top), x.repeat(40, 1), ids.repeat(40), n_top)
+        t = torch.tensor([0.0, -1.0, 0.3, 2.0], device=device).repeat(x.shape[0])[:x.shape[0]]
+        t = torch.where((x == torch.finfo(dtype).min).any(1), 1.0, t)     # (low - max) / T leaves the range of fp32 there
+        compare(score.token_logprobs(x, ids, n_top, temperature=t), x, ids, n_top, t)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_candidates(device, dtype):
+    """The largest scores side by side, and more ties than a list of candidates holds."""
+    V = 40000
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(5, V, generator=g)
+    x[0] = torch.arange(V).float() / 300                              # ascending
+    x[1] = -torch.arange(V).float() / 300
+    x[2, 5000:9000] = 4.5                                             # thousands of ties above everything
+    x[3] = torch.where(torch.rand(V, generator=g) < 0.2, 3.0, -1.0)
+    x[4] = torch.arange(V).float() % 8
+    x, ids = x.to(dtype).to(device), torch.tensor([V - 1, 0, 7000, 3, 7]).to(device)
+    for n_top in (1, 20, 128):
+        compare(score.token_logprobs(x, ids, n_top), x, ids, n_top)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_strides_and_types(device):
+    x, ids, t = rows(6, 500, torch.bfloat16, 2, device, 9)
+    want = score.token_logprobs(x.contiguous(), ids, 4, temperature=t)
+    wide = torch.zeros(12, dtype=torch.int64, device=device)
+    wide[::2] = ids
+    wide_t = torch.ones(18, device=device)
+    wide_t[::3] = t
+    for a, b in zip(want, score.token_logprobs(x, wide[::2], 4, temperature=wide_t[::3])):
+        assert torch.equal(a, b)
+    every = x.contiguous().repeat_interleave(2, 0)
+    for a, b in zip(want, score.token_logprobs(every[::2], ids, 4, temperature=t)):
+        assert torch.equal(a, b)
+    same = x[:1].expand(6, -1)                                        # rows of stride 0
+    got = score.token_logprobs(same, ids, 2)
+    compare(got, same, ids, 2)
+    half = (torch.randn(3, 400, generator=torch.Generator().manual_seed(1)) * 2).half().to(device)
+    compare(score.token_logprobs(half, ids[:3] % 400, 3), half, ids[:3] % 400, 3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_rows(device):
+    x = torch.empty(0, 50, device=device)
+    ids = torch.empty(0, dtype=torch.int64, device=device)
+    got = score.token_logprobs(x, ids, 3)
+    assert [tuple(g.shape) for g in got] == [(0,), (0,), (0, 3), (0, 3)]
+    h, w = torch.empty(0, 64, dtype=torch.bfloat16, device=device), torch.zeros(50, 64, dtype=torch.bfloat16, device=device)
+    assert [tuple(g.shape) for g in score.head_logprobs(h, w, ids)] == [(0,), (0,)]
+
+
+def test_refusals():
+    x, ids = torch.zeros(4, 30), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        score.token_logprobs(x, ids, 31)
+    with pytest.raises(ValueError):
+        score.token_logprobs(x, ids, -1)
+    with pytest.raises(ValueError):
+        score.token_logprobs(torch.zeros(2, 500), ids[:2], 129)
+    with pytest.raises(ValueError):
+        score.token_logprobs(x.T, torch.zeros(30, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        score.token_logprobs(x[0], ids)
+    with pytest.raises(ValueError):
+        score.token_logprobs(x[:, :0], ids)
+    with pytest.raises(TypeError):
+        score.token_logprobs(x, ids.int())
+    with pytest.raises(TypeError):
+        score.token_logprobs(x, ids[:3])
+    with pytest.raises(TypeError):
+        score.token_logprobs(x, ids, temperature=torch.ones(3))
+    with pytest.raises(TypeError):
+        score.token_logprobs(x, ids, temperature=torch.ones(4, dtype=torch.float64))
+    h, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(9, 16, dtype=torch.bfloat16)
+    for bad in (w[:, :8], w.float(), w.T, w[:0], w[0]):
+        with pytest.raises(ValueError):
+            score.head_logprobs(h, bad, ids)
+    with pytest.raises(TypeError):
+        score.head_logprobs(h, w, ids[:2])
+
+
+def test_bounds_check(monkeypatch):
+    from xllm_b200.ops._debug import BoundsError
+    monkeypatch.setenv("XLLM_BOUNDS_CHECK", "1")
+    x = torch.zeros(2, 30)
+    score.token_logprobs(x, torch.tensor([-1, 29]))
+    with pytest.raises(BoundsError):
+        score.token_logprobs(x, torch.tensor([0, 30]))
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    h, w = torch.zeros(4, 20, dtype=torch.bfloat16, device="cuda"), torch.zeros(9, 20, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        score.head_logprobs(h, w, ids)                                # a width that is no multiple of 8
+    with pytest.raises(ValueError):
+        score.head_logprobs(h[:, 1:17], w[:, 1:17], ids)              # rows off the 16-byte boundaries
+    with pytest.raises(ValueError):
+        score.head_logprobs(h[:, :16].float(), w[:, :16].float(), ids)
+    with pytest.raises(TypeError):
+        score.token_logprobs(h, ids.cpu())
+    with pytest.raises(ValueError):
+        score.head_logprobs(h[:, :16].contiguous(), w[:, :16].contiguous().cpu(), ids)
+
+
+# ------------------------------------------------------------------------------- from hidden states
+def head_case(T, K, V, seed, device, spread=1.4):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, K, generator=g) * spread / math.sqrt(K)).to(torch.bfloat16)
+    ids = torch.randint(0, V, (T,), generator=g)
+    h = (torch.randn(T, K, generator=g) + torch.rand(T, 1, generator=g) * 3 * w[ids].float()).to(torch.bfloat16)
+    t = torch.rand(T, generator=g) * 1.5 + 0.3
+    return h.to(device), w.to(device), ids.to(device), t.to(device)
+
+
+def compare_head(got, h, w, ids, temperature=None):
+    """A score is a sum of K exact products: off by at most 2^-23 of the sum of their sizes an addition, truncated.  A
+    log-probability moves by at most twice as much as the scores, the entropy H by at most 2 H times."""
+    x = h.double().cpu() @ w.double().cpu().T
+    size = (h.double().cpu().abs() @ w.double().cpu().abs().T).amax(1)
+    T = torch.ones(len(x)).double() if temperature is None else temperature.double().cpu()
+    off = h.shape[1] * 2.0 ** -23 * size / torch.where(T > 0, T, 1.0)
+    lp, ent, _, _, far = exact(x, ids, 0, temperature)
+    V = w.shape[0]
+    unit = STEP * (V / 128 + 64)
+    near(got[0], lp, 2 * off + unit * (1 + far + math.log(V)), "logprob")
+    near(got[1], ent, (2 * off + 2 * unit) * (1 + math.log(V)), "entropy")
+    assert got[0].dtype == got[1].dtype == torch.float32
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,K,V", [(1, 8, 1), (1, 64, 17), (3, 72, 300), (5, 200, 513), (64, 64, 255), (129, 136, 256), (257, 64, 1031),
+                                   (2, 1000, 4099)])
+def test_head(device, T, K, V):
+    h, w, ids, t = head_case(T, K, V, T + K + V, device)
+    compare_head(score.head_logprobs(h, w, ids), h, w, ids)
+    compare_head(score.head_logprobs(h, w, ids, temperature=t), h, w, ids, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,V", [(1, 4096, 151936), (16, 512, 50257), (32, 2048, 32000), (45, 1024, 129280), (100, 512, 32003), (130, 512, 32768),
+                                   (300, 2880, 9000), (1000, 256, 40000), (4097, 128, 12345)])
+def test_head_sizes(T, K, V):
+    h, w, ids, t = head_case(T, K, V, 7, "cuda")
+    got = score.head_logprobs(h, w, ids, temperature=t)
+    at = torch.tensor(sorted({0, T // 2, T // 3, T - 1}), device="cuda")
+    compare_head(tuple(g[at] for g in got), h[at], w, ids[at], t[at])
+    assert score.error_status() == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_head_edges(device):
+    h, w, ids, t = head_case(12, 64, 700, 3, device)
+    ids[0], ids[1], ids[2] = -1, 700, 699
+    t[3], t[4] = 0.0, -2.0
+    h[5] = 0                                                          # every score alike
+    h[6] *= 40                                                        # one token certain
+    compare_head(score.head_logprobs(h, w, ids, temperature=t), h, w, ids, t)
+    h[7, 3], h[8, 5] = math.nan, math.inf
+    w[11, 5] = w[:, 5].abs().max()                                    # a positive weight: some score is +inf
+    got = score.head_logprobs(h, w, ids)
+    assert torch.isnan(got[0][7:9]).all() and torch.isnan(got[1][7:9]).all()
+    keep = torch.tensor([i for i in range(12) if i not in (7, 8)], device=device)
+    compare_head(tuple(g[keep] for g in got), h[keep], w, ids[keep])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_head_strides(device):
+    h, w, ids, t = head_case(9, 128, 333, 4, device)
+    want = score.head_logprobs(h, w, ids, temperature=t)
+    wide_h, wide_w = torch.full((9, 200), math.nan, dtype=h.dtype, device=device), torch.full((400, 136), math.nan, dtype=h.dtype, device=device)
+    wide_h[:, 8:136], wide_w[:333, :128] = h, w
+    for a, b in zip(want, score.head_logprobs(wide_h[:, 8:136], wide_w[:333, :128], ids, temperature=t)):
+        assert torch.equal(a, b)
+    same = h[:1].expand(9, -1)
+    compare_head(score.head_logprobs(same, w, ids), same, w, ids)
+
+
+@pytest.mark.gpu
+def test_bits_repeat_and_streams():
+    """The same call gives the same bits, on a stream of its own too, and beside another one."""
+    x, ids, t = rows(5, 30000, torch.bfloat16, 8, "cuda")
+    h, w, hid, ht = head_case(70, 256, 20000, 8, "cuda")
+    a, b = score.token_logprobs(x, ids, 9, temperature=t), score.head_logprobs(h, w, hid, temperature=ht)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append((score.token_logprobs(x, ids, 9, temperature=t), score.head_logprobs(h, w, hid, temperature=ht)))
+    torch.cuda.synchronize()
+    for c, d in got:
+        assert all(torch.equal(p, q) for p, q in zip(a, c)) and all(torch.equal(p, q) for p, q in zip(b, d))
+
+
+@pytest.mark.gpu
+def test_captured():
+    """Two graphs, replayed after each other with other inputs in the same places."""
+    from xllm_b200.ops import gemm_tcgen05
+    gemm_tcgen05.prepare()
+    x, ids, t = rows(40, 5000, torch.bfloat16, 8, "cuda")
+    h, w, hid, ht = head_case(33, 128, 3000, 9, "cuda")
+    call = [lambda: score.token_logprobs(x, ids, 5, temperature=t), lambda: score.head_logprobs(h, w, hid, temperature=ht)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for f in call:
+            f()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for f in call + call:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f()
+        graphs.append((g, out, f))
+    x2, ids2, _ = rows(40, 5000, torch.bfloat16, 18, "cuda")
+    h2, _, hid2, _ = head_case(33, 128, 3000, 19, "cuda")
+    x.copy_(x2), ids.copy_(ids2), h.copy_(h2), hid.copy_(hid2)
+    for g, _, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for _, out, f in graphs:
+        for a, b in zip(out, f()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits():
+    """Row offsets that pass 2^31 elements."""
+    V = 151936
+    n = (1 << 31) // V + 3
+    x = torch.zeros(n, V, dtype=torch.bfloat16, device="cuda")
+    y, ids, _ = rows(3, V, torch.bfloat16, 6, "cuda")
+    x[-3:] = y
+    every = torch.zeros(n, dtype=torch.int64, device="cuda")
+    every[-3:] = ids
+    got = score.token_logprobs(x, every, 2)
+    compare(tuple(g[-3:] for g in got), y, ids, 2)
+    assert abs(float(got[0][0]) + math.log(V)) < 1e-4 and got[2][0].tolist() == [0, 1]

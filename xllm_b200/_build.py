@@ -45,9 +45,9 @@ NVCC_FLAGS = [
     "-I", str(CSRC),
 ]
 # Sources built without --use_fast_math: their exponentials feed recurrences (errors of a decay multiply up over a
-# sequence) or serve the fp32 execution type.
+# sequence), serve the fp32 execution type or give results in fp32.
 PRECISE_SOURCES = {"linear_attn", "residual", "rope_norm_kv", "attn_generic", "delta_rule", "mlstm", "head_norm", "proj_f32", "moe",
-                   "gdn_layer"}
+                   "gdn_layer", "logprobs", "head_logprobs"}
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-pthread",
              "-I", str(CSRC / "runtime"), "-I", str(CSRC / "frontend"), "-I", str(CSRC / "server"),
              "-Wall", "-Wno-sign-compare", "-I", str(CSRC), "-I", "/usr/local/cuda/include"]

@@ -1,0 +1,59 @@
+// Softmax statistics that the scoring kernels share.  A tally of some scores x under the factor c = log2(e) / temperature:
+//
+//   m = max x        z = sum 2^t        s = sum 2^t t        with t = (x - m) c
+//
+// so that of a whole row   log softmax(x[i]) = (x[i] - m) / temperature - log z   and the entropy in bits is   log2 z - s / z.
+// Everything is relative to m, where fp32 loses nothing: the sums of terms relative to 0 would cancel.
+// -inf adds nothing; NaN and +inf make z NaN, and with it every result of the row.  The tally of nothing is {-FLT_MAX, 0, 0}.
+#pragma once
+#include <cfloat>
+
+#include "common.cuh"
+
+namespace xllm {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Tally {
+  float m, z, s;
+};
+
+__device__ __forceinline__ float exp2_fast(float t) {          // 2^-22 relative, 0 below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+// t from below so that 0 * -inf does not meet in s; NaN stays NaN
+__device__ __forceinline__ float bounded(float t) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(t), "f"(-1024.f));
+  return r;
+}
+__device__ __forceinline__ Tally tally_empty() { return {-FLT_MAX, 0.f, 0.f}; }
+// the same tally relative to a maximum m >= a.m
+__device__ __forceinline__ void tally_rebase(Tally& a, float m, float c) {
+  const float d = bounded((a.m - m) * c), f = exp2_fast(d);
+  a.s = f * fmaf(d, a.z, a.s);
+  a.z *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Tally tally_join(Tally a, Tally b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  tally_rebase(a, m, c);
+  tally_rebase(b, m, c);
+  return {m, a.z + b.z, a.s + b.s};
+}
+// 1 / temperature of a row; c is log2(e) times it
+__device__ __forceinline__ float row_scale(const float* temperature, int64_t row) {
+  const float t = temperature ? temperature[row] : 1.f;
+  return t > 0.f ? 1.f / t : 1.f;
+}
+// in nats: the type's lowest value as a score leaves fp32's range when scaled to bits
+__device__ __forceinline__ float tally_logprob(const Tally& a, float x, float scale) {
+  return a.z == 0.f ? -INFINITY : (x - a.m) * scale - logf(a.z);
+}
+__device__ __forceinline__ float tally_entropy(const Tally& a) {
+  return a.z == 0.f ? 0.f : (log2f(a.z) - a.s / a.z) * kLn2;
+}
+
+}  // namespace xllm
