@@ -178,11 +178,11 @@ def test_strides_and_types(device):
     wide[::2] = ids
     wide_t = torch.ones(18, device=device)
     wide_t[::3] = t
-    for a, b in zip(want, score.token_logprobs(x, wide[::2], 4, temperature=wide_t[::3])):
-        assert torch.equal(a, b)
+    # a row that starts elsewhere within 16 bytes is summed in another order, so not to the same bits: each is within the bound
+    compare(want, x, ids, 4, t)
+    compare(score.token_logprobs(x, wide[::2], 4, temperature=wide_t[::3]), x, ids, 4, t)
     every = x.contiguous().repeat_interleave(2, 0)
-    for a, b in zip(want, score.token_logprobs(every[::2], ids, 4, temperature=t)):
-        assert torch.equal(a, b)
+    compare(score.token_logprobs(every[::2], ids, 4, temperature=t), x, ids, 4, t)
     same = x[:1].expand(6, -1)                                        # rows of stride 0
     got = score.token_logprobs(same, ids, 2)
     compare(got, same, ids, 2)
