@@ -43,6 +43,49 @@ __device__ __forceinline__ Tally tally_join(Tally a, Tally b, float c) {
   tally_rebase(b, m, c);
   return {m, a.z + b.z, a.s + b.s};
 }
+// Pairs of fp32 in one instruction.
+struct f32x2 {
+  float x, y;
+};
+#define XLLM_F32X2(name, op)                                                                                         \
+  __device__ __forceinline__ f32x2 name(f32x2 a, f32x2 b) {                                                          \
+    f32x2 r;                                                                                                         \
+    asm("{\n\t.reg .b64 p, q, s;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\t" op                             \
+        " s, p, q;\n\tmov.b64 {%0, %1}, s;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));   \
+    return r;                                                                                                        \
+  }
+XLLM_F32X2(add2, "add.rn.f32x2")
+XLLM_F32X2(mul2, "mul.rn.f32x2")
+#undef XLLM_F32X2
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("{\n\t.reg .b64 p, q, s, t;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 s, {%6, %7};\n\t"
+      "fma.rn.f32x2 t, p, q, s;\n\tmov.b64 {%0, %1}, t;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// A tally that takes two scores at a time: its sums are those of the first and of the second ones.
+struct PairTally {
+  float m;
+  f32x2 z, s;
+};
+__device__ __forceinline__ PairTally pair_empty() { return {-FLT_MAX, {0.f, 0.f}, {0.f, 0.f}}; }
+__device__ __forceinline__ void pair_rebase(PairTally& a, float m, float c) {      // m >= a.m
+  const float d = bounded((a.m - m) * c), f = exp2_fast(d);
+  a.s = mul2({f, f}, fma2({d, d}, a.z, a.s));
+  a.z = mul2({f, f}, a.z);
+  a.m = m;
+}
+__device__ __forceinline__ void pair_add(PairTally& a, f32x2 x, float c) {         // neither is above a.m
+  f32x2 t = mul2(add2(x, {-a.m, -a.m}), {c, c});
+  t = {bounded(t.x), bounded(t.y)};
+  const f32x2 e = {exp2_fast(t.x), exp2_fast(t.y)};
+  a.z = add2(a.z, e);
+  a.s = fma2(e, t, a.s);
+}
+__device__ __forceinline__ Tally pair_sum(const PairTally& a) { return {a.m, a.z.x + a.z.y, a.s.x + a.s.y}; }
+
 // 1 / temperature of a row; c is log2(e) times it
 __device__ __forceinline__ float row_scale(const float* temperature, int64_t row) {
   const float t = temperature ? temperature[row] : 1.f;

@@ -10,6 +10,7 @@
 // (score, lowest index first) is the number of listed ones in front of it.  A list that overflows (thousands of ties, or
 // scores in ascending order) is made by one pass over the part for each place instead.
 #include "logprob_math.cuh"
+#include "tc_common.cuh"
 #include "vec_io.cuh"
 
 namespace xllm {
@@ -40,28 +41,6 @@ __device__ __forceinline__ float key_score(uint64_t k) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
-
-// Pairs of fp32 in one instruction.
-struct f32x2 {
-  float x, y;
-};
-#define XLLM_F32X2(name, op)                                                                                         \
-  __device__ __forceinline__ f32x2 name(f32x2 a, f32x2 b) {                                                          \
-    f32x2 r;                                                                                                         \
-    asm("{\n\t.reg .b64 p, q, s;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\t" op                             \
-        " s, p, q;\n\tmov.b64 {%0, %1}, s;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));   \
-    return r;                                                                                                        \
-  }
-XLLM_F32X2(add2, "add.rn.f32x2")
-XLLM_F32X2(mul2, "mul.rn.f32x2")
-#undef XLLM_F32X2
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("{\n\t.reg .b64 p, q, s, t;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 s, {%6, %7};\n\t"
-      "fma.rn.f32x2 t, p, q, s;\n\tmov.b64 {%0, %1}, t;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
 
 // One 16-byte vector of scores.
 template <typename T>
@@ -121,22 +100,9 @@ __device__ __forceinline__ Tally block_tally(Tally a, float c, Tally* red) {
   return a;
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_block(const void* p, uint32_t rank) {       // the same place in another block
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
 __device__ __forceinline__ float remote_f32(uint32_t a) {
@@ -168,7 +134,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) token_logprobs_kernel(ScoreP
   constexpr int U = 4;
   __shared__ ScoreShared sh;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int split = (int)cluster_size(), part = (int)cluster_rank();
+  const int split = (int)cluster_size(), part = (int)tc::cluster_rank();
   const int row = blockIdx.x / split;
   pdl_wait();
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.row_stride;
@@ -181,8 +147,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) token_logprobs_kernel(ScoreP
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   const int single = part == 0 && tid < head ? tid : part == split - 1 && tid >= 32 && tail + tid - 32 < p.V ? tail + tid - 32 : -1;
 
-  Tally a = tally_empty();
-  f32x2 z = {0.f, 0.f}, s = {0.f, 0.f};
+  PairTally run = pair_empty();
   for (int j = v0 + tid; j < v1; j += kScoreThreads * U) {
     Vec v[U];
 #pragma unroll
@@ -192,27 +157,13 @@ __global__ void __launch_bounds__(kScoreThreads, 5) token_logprobs_kernel(ScoreP
       else v[u].nothing();
     }
     const float m = vec_max<U>(v);
-    if (m > a.m) {
-      const float d = bounded((a.m - m) * c), f = exp2_fast(d);
-      const f32x2 ff = {f, f};
-      s = mul2(ff, fma2({d, d}, z, s));
-      z = mul2(ff, z);
-      a.m = m;
-    }
-    const f32x2 nm = {-a.m, -a.m}, cc = {c, c};
+    if (m > run.m) pair_rebase(run, m, c);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < Vec::N / 2; ++i) {
-        f32x2 t = mul2(add2(v[u].pair(i), nm), cc);
-        t = {bounded(t.x), bounded(t.y)};
-        const f32x2 e = {exp2_fast(t.x), exp2_fast(t.y)};
-        z = add2(z, e);
-        s = fma2(e, t, s);
-      }
+      for (int i = 0; i < Vec::N / 2; ++i) pair_add(run, v[u].pair(i), c);
   }
-  a.z = z.x + z.y;
-  a.s = s.x + s.y;
+  Tally a = pair_sum(run);
   if (single >= 0) tally_add(a, to_f32(x[single]), c);
 
   const int n = p.n_top;
@@ -307,15 +258,15 @@ __global__ void __launch_bounds__(kScoreThreads, 5) token_logprobs_kernel(ScoreP
 
   if (split > 1) {
     if (tid == 0) sh.part = a;
-    cluster_sync();
+    tc::cluster_sync();
     if (part == 0) {
       a = tally_empty();
       for (int r = 0; r < split; ++r) {
-        const uint32_t at = in_block(&sh.part, r);
+        const uint32_t at = tc::in_cta(smem_u32(&sh.part), r);
         a = tally_join(a, {remote_f32(at), remote_f32(at + 4), remote_f32(at + 8)}, c);
       }
       if constexpr (TOP) {
-        for (int i = tid; i < split * n; i += kScoreThreads) sh.listed[i] = remote_u64(in_block(sh.top + i % n, i / n));
+        for (int i = tid; i < split * n; i += kScoreThreads) sh.listed[i] = remote_u64(tc::in_cta(smem_u32(sh.top + i % n), i / n));
         __syncthreads();
         uint64_t mine[kScoreListed / kScoreThreads];
         int place[kScoreListed / kScoreThreads];
@@ -329,17 +280,17 @@ __global__ void __launch_bounds__(kScoreThreads, 5) token_logprobs_kernel(ScoreP
             for (int k = 0; k < split * n; ++k) place[q] += sh.listed[k] > mine[q];
           }
         }
-        cluster_sync();                              // the others' places have been read; every block passes here once
+        tc::cluster_sync();                              // the others' places have been read; every block passes here once
         if (tid < n) sh.top[tid] = 0;
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < kScoreListed / kScoreThreads; ++q)
           if (mine[q] != 0 && place[q] < n) sh.top[place[q]] = mine[q];
       } else {
-        cluster_sync();
+        tc::cluster_sync();
       }
     } else {
-      cluster_sync();
+      tc::cluster_sync();
       return;
     }
   }

@@ -154,6 +154,11 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_on(index: int):
+    """The current stream of device `index`, without the stream object of `stream()` (3 us of a short call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def check(rc: int, name: str):
     if rc != 0:
         raise RuntimeError(f"{name} failed with CUDA error {rc}")

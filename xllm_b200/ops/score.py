@@ -13,8 +13,8 @@ from __future__ import annotations
 
 import torch
 
-from . import _debug, _lib
-from ._lib import I, L, P, check, ptr, stream
+from . import _count, _debug, _lib
+from ._lib import I, L, P, check, ptr, stream_on
 
 _lib.register_signature("xllm_token_logprobs", [P, L, I, I, I, P, P, I, P, P, P, P, P])
 _lib.register_signature("xllm_head_logprobs", [P, L, P, L, I, I, I, P, P, P, P, P, P])
@@ -55,13 +55,20 @@ def token_logprobs_reference(logits, ids, n_top=0, temperature=None):
 
 
 def _check_rows(x, ids, temperature, name):
-    if x.dim() != 2 or x.stride(-1) != 1 and x.shape[-1] > 1:
+    """Refuses what no kernel reads; returns the rows' device."""
+    dev = x.device
+    if x.dim() != 2 or x.stride(1) != 1 and x.shape[1] > 1:
         raise ValueError(f"{name}: rows [rows, columns] with adjacent columns expected, got {tuple(x.shape)} strides {x.stride()}")
-    if ids.dtype != torch.int64 or ids.shape != x.shape[:1] or ids.device != x.device:
-        raise TypeError(f"{name}: ids are int64 [{x.shape[0]}] on {x.device}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-    if temperature is not None and (temperature.dtype != torch.float32 or temperature.shape != x.shape[:1]
-                                    or temperature.device != x.device):
-        raise TypeError(f"{name}: temperatures are fp32 [{x.shape[0]}] on {x.device}")
+    rows = x.shape[:1]
+    if ids.dtype != torch.int64 or ids.shape != rows or ids.device != dev:
+        raise TypeError(f"{name}: ids are int64 [{x.shape[0]}] on {dev}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+    if temperature is not None and (temperature.dtype != torch.float32 or temperature.shape != rows or temperature.device != dev):
+        raise TypeError(f"{name}: temperatures are fp32 [{x.shape[0]}] on {dev}")
+    return dev
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def token_logprobs(logits, ids, n_top=0, temperature=None):
@@ -69,32 +76,30 @@ def token_logprobs(logits, ids, n_top=0, temperature=None):
     [rows] or None.  Returns (logprob fp32 [rows], entropy fp32 [rows], alternatives int32 [rows, n_top], their
     log-probabilities fp32 [rows, n_top]); the alternatives are the n_top largest logits, largest first, ties to the lowest index, -1 and
     -inf where the row has no more tokens above -inf, and None without n_top."""
-    _check_rows(logits, ids, temperature, "token_logprobs")
+    dev = _check_rows(logits, ids, temperature, "token_logprobs")
     rows, vocab = logits.shape
     if vocab < 1 or not 0 <= n_top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_logprobs: 0 to {min(MAX_TOP, vocab)} alternatives of a vocabulary of {vocab}, asked for {n_top}")
-    _debug.check_range(ids, 0, vocab, "token_logprobs ids", allow_negative_skip=True)
+    if _debug.enabled():
+        _debug.check_range(ids, 0, vocab, "token_logprobs ids", allow_negative_skip=True)
     if not logits.is_cuda:
         return token_logprobs_reference(logits, ids, n_top, temperature)
     dt = 0 if logits.dtype == torch.bfloat16 else 1
     if dt == 1 and logits.dtype != torch.float32:
         logits = logits.float()
-    dev = logits.device
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return token_logprobs(logits, ids, n_top, temperature)
-    ids = ids if ids.is_contiguous() else ids.contiguous()
-    if temperature is not None and not temperature.is_contiguous():
-        temperature = temperature.contiguous()
+    ids, temperature = _dense(ids), _dense(temperature)
     lp = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(lp)
     top = top_lp = None
     if n_top:
         top = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
-        top_lp = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
+        top_lp = lp.new_empty((rows, n_top))
     check(_lib.load().xllm_token_logprobs(ptr(logits), logits.stride(0), dt, rows, vocab, ptr(ids), ptr(temperature), int(n_top),
-                                          ptr(lp), ptr(entropy), ptr(top), ptr(top_lp), stream()), "token_logprobs")
-    from . import _count
+                                          ptr(lp), ptr(entropy), ptr(top), ptr(top_lp), stream_on(index)), "token_logprobs")
     _count()
     return lp, entropy, top, top_lp
 
@@ -103,10 +108,15 @@ def head_logprobs_reference(hidden, weight, ids, temperature=None):
     return token_logprobs_reference(hidden.float() @ weight.float().T, ids, 0, temperature)[:2]
 
 
+def _stride(t):
+    """Elements between rows; a single row has none of its own."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def head_supported(hidden, weight):
     """Whether `head_logprobs` takes these on CUDA: bf16, rows of 16-byte multiples that start on such a boundary."""
-    return (hidden.is_cuda and hidden.dtype == weight.dtype == torch.bfloat16 and hidden.shape[-1] % 8 == 0
-            and hidden.stride(0) % 8 == 0 and weight.stride(0) % 8 == 0 and not (hidden.data_ptr() | weight.data_ptr()) & 15)
+    return (hidden.is_cuda and hidden.dtype == weight.dtype == torch.bfloat16 and hidden.shape[1] % 8 == 0
+            and not (_stride(hidden) | _stride(weight)) % 8 and not (hidden.data_ptr() | weight.data_ptr()) % 16)
 
 
 def head_logprobs(hidden, weight, ids, temperature=None):
@@ -114,33 +124,35 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     and weight [vocab, width] bf16, the products' sums fp32 and never rounded to bf16 (so not the bits of the two steps, which
     round every logit).  Returns (logprob, entropy) fp32 [rows].  On CUDA the width is a multiple of 8 and rows start on
     16-byte boundaries."""
-    _check_rows(hidden, ids, temperature, "head_logprobs")
+    dev = _check_rows(hidden, ids, temperature, "head_logprobs")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.stride(-1) != 1 or weight.dtype != hidden.dtype \
             or weight.shape[0] < 1 or weight.device != hidden.device:
         raise ValueError(f"head_logprobs: weight [vocab, {hidden.shape[1]}] {hidden.dtype} on {hidden.device} expected, got "
                          f"{tuple(weight.shape)} {weight.dtype} on {weight.device}")
     rows, width = hidden.shape
     vocab = weight.shape[0]
-    _debug.check_range(ids, 0, vocab, "head_logprobs ids", allow_negative_skip=True)
+    if _debug.enabled():
+        _debug.check_range(ids, 0, vocab, "head_logprobs ids", allow_negative_skip=True)
     if not hidden.is_cuda:
         return head_logprobs_reference(hidden, weight, ids, temperature)
     if not head_supported(hidden, weight):
         raise ValueError(f"head_logprobs: bf16 with a width in multiples of 8 and 16-byte aligned rows expected, got {hidden.dtype} "
                          f"{tuple(hidden.shape)} strides {hidden.stride()}, weight strides {weight.stride()}")
-    dev = hidden.device
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return head_logprobs(hidden, weight, ids, temperature)
-    ids = ids if ids.is_contiguous() else ids.contiguous()
-    if temperature is not None and not temperature.is_contiguous():
-        temperature = temperature.contiguous()
+    ids, temperature = _dense(ids), _dense(temperature)
+    if _stride(hidden) < width:                     # one row for all, or overlapping ones
+        hidden = hidden.contiguous()
+    if _stride(weight) < width:
+        weight = weight.contiguous()
     lib = _lib.load()
     lp = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(lp)
     work = torch.empty(lib.xllm_head_logprobs_workspace(rows, vocab), dtype=torch.uint8, device=dev)
-    check(lib.xllm_head_logprobs(ptr(hidden), hidden.stride(0), ptr(weight), weight.stride(0), rows, vocab, width, ptr(ids),
-                                 ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream()), "head_logprobs")
-    from . import _count
+    check(lib.xllm_head_logprobs(ptr(hidden), _stride(hidden), ptr(weight), _stride(weight), rows, vocab, width, ptr(ids),
+                                 ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream_on(index)), "head_logprobs")
     _count(2)
     return lp, entropy
 

@@ -8,8 +8,8 @@ from typing import NamedTuple
 
 import torch
 
-from . import _debug, _lib
-from ._lib import I, L, P, check, ptr, stream
+from . import _count, _debug, _lib
+from ._lib import I, L, P, check, ptr, stream_on
 
 _lib.register_signature("xllm_step_tables", [P, L, I, I, P, P, I, I, P, I, P, P, P, P, P, P, P])
 
@@ -82,18 +82,20 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
     if not block_table.is_cuda:
         free = free_blocks if free_blocks is not None else torch.empty(0, dtype=torch.int32)
         return step_tables_reference(block_table, ctx_lens, q_lens, page, n_rows, free)
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks)
     ctx_lens, q_lens = ctx_lens.contiguous(), q_lens.contiguous()
-    free_blocks = None if free_blocks is None else free_blocks.contiguous()
-    out = StepTables(torch.empty(B + 1, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev),
-                     torch.empty(n_rows, dtype=torch.int64, device=dev), torch.empty(n_rows, dtype=torch.int32, device=dev),
-                     torch.empty(B, dtype=torch.int64, device=dev), torch.empty((), dtype=torch.int32, device=dev))
+    n_free = 0
+    if free_blocks is not None:
+        free_blocks, n_free = free_blocks.contiguous(), free_blocks.shape[0]
+    # one allocation for each type: half a step's time is the host's
+    cu_q, kv_lens, slots, taken = torch.empty(2 * B + n_rows + 2, dtype=torch.int32, device=dev).split_with_sizes([B + 1, B, n_rows, 1])
+    positions, last_rows = torch.empty(n_rows + B, dtype=torch.int64, device=dev).split_with_sizes([n_rows, B])
+    out = StepTables(cu_q, kv_lens, positions, slots, last_rows, taken.view(()))
     check(_lib.load().xllm_step_tables(ptr(block_table), block_table.stride(0), B, width, ptr(ctx_lens), ptr(q_lens), int(page),
-                                       int(n_rows), ptr(free_blocks), 0 if free_blocks is None else free_blocks.shape[0],
-                                       ptr(out.cu_q), ptr(out.kv_lens), ptr(out.positions), ptr(out.slots), ptr(out.last_rows),
-                                       ptr(out.taken), stream()), "step_tables")
-    from . import _count
+                                       int(n_rows), ptr(free_blocks), n_free, ptr(cu_q), ptr(kv_lens), ptr(positions), ptr(slots),
+                                       ptr(last_rows), ptr(taken), stream_on(index)), "step_tables")
     _count()
     return out
