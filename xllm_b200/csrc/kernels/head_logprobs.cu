@@ -5,10 +5,12 @@
 //                      columns, and the given token's score from whichever tile holds it
 //   head_join_kernel   a row's tallies over all tiles, joined in a fixed order
 //
-// A tile is a pair of CTAs' (cta_group::2): each loads its 128 rows of h and half of the columns' rows of W by TMA into a ring
-// of stages, one thread of the pair's first CTA issues the products into one of two accumulators in tensor memory, and four warps
-// of each CTA read the other one back, a thread a row, 32 columns at a time.  Few rows are bound by W's way from HBM, many
-// by the tensor cores; the tally (some 6 instructions a score, 2000 cycles a tile) hides behind the next tile's products from a width of 256 on.
+// Many rows: a tile is a pair of CTAs' (cta_group::2), each loads its 128 rows of h and half of the columns' rows of W by TMA into
+// a ring of stages, one thread of the pair's first CTA issues the products into one of two accumulators in tensor memory, and eight
+// warps of each CTA read the other one back, two threads a row, 32 columns at a time.  Bound by the tensor cores; the tally (some
+// 3000 cycles a tile) hides behind the next tile's products where K is 512 and more.
+// Up to 128 rows: a tile is one CTA's and bound by W's way from HBM.  An SM's share of the bandwidth depends on its die (of two
+// equal shares one was read in 176 us, the other in 203), so a CTA that is done takes over one that has not started.
 //
 // Every wait is bounded; on expiry the kernel raises an error word, all roles leave their loops, tensor memory is freed and the
 // kernel returns.
@@ -21,22 +23,28 @@ namespace xllm {
 using namespace tc;
 
 constexpr int kHeadRows = 128, kHeadCols = 256, kHeadK = 64;        // rows of a CTA, most columns of a tile, a K block
-constexpr int kHeadStages = 7, kHeadThreads = 192;
-constexpr int kHeadABytes = kHeadRows * kHeadK * 2, kHeadBBytes = kHeadCols / 2 * kHeadK * 2;
-constexpr int kHeadStageBytes = kHeadABytes + kHeadBBytes;
-constexpr int kHeadBarOff = kHeadStages * kHeadStageBytes;
-constexpr int kHeadSmem = kHeadBarOff + (2 * kHeadStages + 4) * 8 + 16 + 1024;
+constexpr int kHeadWarps = 8, kHeadThreads = 64 + 32 * kHeadWarps, kHeadMostStages = 16;
+constexpr int kHeadRing = 7 * 32 * 1024;                            // bytes of the ring of stages
+constexpr int kHeadBars = 2 * kHeadMostStages + 8;
+constexpr int kHeadFixed = 2 * 16 + kHeadBars * 8 + 16;                // behind it: answers, barriers, two words; then tallies of 128 rows
+constexpr int kHeadSmem = kHeadRing + kHeadFixed + kHeadRows * sizeof(Tally) + 1024;
 static_assert(kHeadSmem <= 232448, "exceeds the 227 KB of shared memory per CTA");
 
 __device__ int g_head_error = 0;
 
-// workspace: tallies [column tiles][rows] and the given tokens' scores [rows]
+// workspace: tallies (m, z, s, -) [rows][column tiles] and the given tokens' scores [rows], as the tensor cores and as fp32 sums give them
 struct HeadParams {
-  int T, V, K, cols, n_tiles, m_tiles, a_box;
+  int T, V, K, cols, n_tiles, m_tiles;
+  int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
+  const bf16* h;
+  int64_t ldh;
+  const bf16* w;
+  int64_t ldw;
   const int64_t* ids;
   const float* temperature;
-  Tally* tallies;
+  float4* tallies;
   float* given;
+  float* summed;
 };
 
 // Tile u of the order in which they are worked on: the row tiles of a column tile side by side, so that W is read from HBM once for
@@ -49,67 +57,110 @@ __device__ __forceinline__ void head_tile(const HeadParams& p, int u, int& m, in
   m = g * kHeadGroup + r - n * wide;
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHeadThreads, 1)
+template <bool PAIR>
+__global__ void __launch_bounds__(kHeadThreads, 1)
 head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const uint32_t sbase = smem_u32(smem), bar0 = sbase + kHeadBarOff;
+  const uint32_t sbase = smem_u32(smem), answer0 = sbase + kHeadRing, bar0 = answer0 + 32;
   const auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  const auto empty_bar = [&](int s) { return bar0 + 8u * (kHeadStages + s); };
-  const auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kHeadStages + a); };
-  const auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kHeadStages + 2 + a); };
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kHeadBarOff + (2 * kHeadStages + 4) * 8);
+  const auto empty_bar = [&](int s) { return bar0 + 8u * (kHeadMostStages + s); };
+  const auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + a); };
+  const auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 2 + a); };
+  const auto next_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 4 + a); };       // an answer has arrived
+  const auto read_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 6 + a); };       // all warps have read it
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kHeadRing + 32 + kHeadBars * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
   const int units = p.m_tiles * p.n_tiles, k_blocks = (p.K + kHeadK - 1) / kHeadK;
+  const int w_rows = PAIR ? p.cols / 2 : p.cols;                                  // of W that this CTA loads for a tile
+  const int a_bytes = p.a_box * kHeadK * 2, block_bytes = a_bytes + w_rows * kHeadK * 2;       // of a K block
+  const int stage_bytes = p.per_stage * block_bytes;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kHeadStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 8);                    // four warps in each CTA of the pair
+      mbar_init(tempty_bar(a), PAIR ? 2 * kHeadWarps : kHeadWarps);
+      mbar_init(next_bar(a), 1);
+      mbar_init(read_bar(a), 2 + kHeadWarps);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();                                     // both CTAs' barriers exist before anything can signal them
+  if constexpr (PAIR) cluster_sync();                 // both CTAs' barriers exist before anything can signal them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   pdl_wait();
   pdl_launch_dependents();                            // after the allocation: what starts early may want tensor memory too
 
+  // The tile behind the t-th one, u, of this CTA or pair, or -1: pairs take turns, a single CTA takes over one that has not started.
+  const auto next_unit = [&](int u, int t, bool& ok) {
+    if constexpr (PAIR) {
+      u += gridDim.x >> 1;
+      return u < units ? u : -1;
+    } else {
+      if (!mbar_wait_warp(next_bar(t & 1), (t >> 1) & 1, abort_flag)) { ok = false; return -1; }
+      const int taken = taken_cta(answer0 + 16 * (t & 1));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the place is written again
+      __syncwarp();
+      if (lane == 0) mbar_arrive(read_bar(t & 1));
+      return taken;
+    }
+  };
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+
   if (warp == 0) {
-    // ------------------------------------------------------------------ loads (both CTAs)
-    const uint32_t bytes = 2u * (p.a_box + p.cols / 2) * kHeadK * 2;
-    int stage = 0;
+    // ------------------------------------------------------------------ loads
+    int stage = 0, t = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int u = pair; u < units && ok; u += n_pairs) {
-      int m, n;
-      head_tile(p, u, m, n);
-      const int m0 = m * 2 * kHeadRows + (int)rank * kHeadRows, n0 = n * p.cols + (int)rank * (p.cols / 2);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!mbar_wait_cluster_warp(empty_bar(stage), phase ^ 1, abort_flag)) { ok = false; break; }
-        const uint32_t dst = sbase + stage * kHeadStageBytes;
+    for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
+      if constexpr (!PAIR) {
+        if (!mbar_wait_warp(read_bar(t & 1), ((t >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(full_bar(stage), bytes);
-          tma_load_2d_pair(dst, &map_h, kb * kHeadK, m0, full_bar(stage));
-          tma_load_2d_pair(dst + kHeadABytes, &map_w, kb * kHeadK, n0, full_bar(stage));
+          mbar_expect_tx(next_bar(t & 1), 16);
+          take_cta(answer0 + 16 * (t & 1), next_bar(t & 1));
         }
         __syncwarp();
-        if (++stage == kHeadStages) { stage = 0; phase ^= 1; }
+      }
+      int m, n;
+      head_tile(p, u, m, n);
+      const int m0 = m * 2 * kHeadRows + (int)rank * kHeadRows, n0 = n * p.cols + (int)rank * w_rows;
+      for (int kb = 0; kb < k_blocks; kb += p.per_stage) {
+        if (!mbar_wait_warp(empty_bar(stage), phase ^ 1, abort_flag)) { ok = false; break; }
+        const int blocks = min(p.per_stage, k_blocks - kb);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(full_bar(stage), (PAIR ? 2u : 1u) * blocks * block_bytes);
+          for (int i = 0; i < blocks; ++i) {
+            const uint32_t dst = sbase + stage * stage_bytes + i * block_bytes;
+            if constexpr (PAIR) {
+              tma_load_2d_pair(dst, &map_h, (kb + i) * kHeadK, m0, full_bar(stage));
+              tma_load_2d_pair(dst + a_bytes, &map_w, (kb + i) * kHeadK, n0, full_bar(stage));
+            } else {
+              tma_load_2d(dst, &map_h, (kb + i) * kHeadK, m0, full_bar(stage));
+              tma_load_2d(dst + a_bytes, &map_w, (kb + i) * kHeadK, n0, full_bar(stage));
+            }
+          }
+        }
+        __syncwarp();
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
     }
     if (!ok) {
@@ -118,66 +169,129 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      // ---------------------------------------------------------------- products (the pair's first CTA)
-      const uint32_t id = idesc_pair(p.cols);
+      // ---------------------------------------------------------------- products (a pair's first CTA)
+      const uint32_t id = PAIR ? idesc_pair(p.cols) : idesc(false, p.cols);
       int stage = 0, t = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int u = pair; u < units && ok; u += n_pairs, ++t) {
+      for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
         const int acc = t & 1;
-        if (!mbar_wait_cluster_warp(tempty_bar(acc), ((t >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        if (!(PAIR ? mbar_wait_cluster_warp(tempty_bar(acc), ((t >> 1) & 1) ^ 1, abort_flag)
+                   : mbar_wait_warp(tempty_bar(acc), ((t >> 1) & 1) ^ 1, abort_flag))) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem_base + acc * kHeadCols;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_cluster_warp(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+        for (int kb = 0; kb < k_blocks; kb += p.per_stage) {
+          if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t at = sbase + stage * kHeadStageBytes;
+          const int blocks = min(p.per_stage, k_blocks - kb);
           if (elect_one()) {
-            const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + kHeadABytes, 16, 1024);
+            for (int i = 0; i < blocks; ++i) {
+              const uint32_t at = sbase + stage * stage_bytes + i * block_bytes;
+              const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + a_bytes, 16, 1024);
 #pragma unroll
-            for (int k = 0; k < kHeadK / 16; ++k) umma_pair(d, a + 2 * k, b + 2 * k, id, (kb | k) != 0);
-            umma_commit_pair(empty_bar(stage));
+              for (int k = 0; k < kHeadK / 16; ++k) {
+                if constexpr (PAIR) umma_pair(d, a + 2 * k, b + 2 * k, id, (kb + i | k) != 0);
+                else umma(d, a + 2 * k, b + 2 * k, id, (kb + i | k) != 0);
+              }
+            }
+            if constexpr (PAIR) umma_commit_pair(empty_bar(stage));
+            else umma_commit(empty_bar(stage));
           }
           __syncwarp();
-          if (++stage == kHeadStages) { stage = 0; phase ^= 1; }
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
-        if (ok && elect_one()) umma_commit_pair(tfull_bar(acc));
+        if (ok && elect_one()) {
+          if constexpr (PAIR) umma_commit_pair(tfull_bar(acc));
+          else umma_commit(tfull_bar(acc));
+        }
         __syncwarp();
       }
     }
   } else {
-    // ------------------------------------------------------------------ tallies (both CTAs), a thread a row
-    const int q = warp & 3;
-    const uint32_t leader_tempty = in_cta(tempty_bar(0), 0);
-    int t = 0;
-    for (int u = pair; u < units; u += n_pairs, ++t) {
-      int m, n;
+    // ------------------------------------------------------------------ tallies, two threads a row: every other 32 columns
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t leader_tempty = PAIR ? in_cta(tempty_bar(0), 0) : 0u;
+    const auto row_of = [&](int m) { return m * 2 * kHeadRows + (int)rank * kHeadRows + q * 32; };
+    // a row's token and temperature are fetched a tile ahead
+    int64_t id_next = -1;
+    float c_next = kLog2e;
+    const auto fetch = [&](int m) {
+      const int row = row_of(m) + lane;
+      id_next = row < p.T ? p.ids[row] : -1;
+      c_next = row < p.T ? row_scale(p.temperature, row) * kLog2e : kLog2e;
+    };
+    int t = 0, m, n;
+    bool ok = true;
+    head_tile(p, first, m, n);
+    fetch(m);
+    for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
       head_tile(p, u, m, n);
-      const int row0 = m * 2 * kHeadRows + (int)rank * kHeadRows + q * 32, row = row0 + lane, n0 = n * p.cols, acc = t & 1;
-      const float c = row < p.T ? row_scale(p.temperature, row) * kLog2e : 1.f;
-      const int64_t want = row < p.T ? p.ids[row] - n0 : -1;
-      if (!mbar_wait_cluster_warp(tfull_bar(acc), (t >> 1) & 1, abort_flag)) break;
+      const int row0 = row_of(m), row = row0 + lane, n0 = n * p.cols, acc = t & 1;
+      const float c = c_next;
+      const int64_t want = id_next - n0;              // the given token's column, if it is one of this tile's
+      if (PAIR && u + (int)(gridDim.x >> 1) < units) {
+        int m1, n1;
+        head_tile(p, u + (gridDim.x >> 1), m1, n1);
+        if (m1 != m) fetch(m1);
+      }
+      // The tensor cores' sums of K products are cut off at every step, some 2^-19 of a large score in all.  While the tile is
+      // computed, the given tokens' scores are summed once more as fp32 products that round: a warp a row, shared out by the tiles.
+      constexpr int warps = PAIR ? 2 * kHeadWarps : kHeadWarps;
+      for (int64_t r = (int64_t)u * warps + (int)rank * kHeadWarps + warp - 2; r < p.T; r += (int64_t)units * warps) {
+        const int64_t id = p.ids[r];
+        if (id < 0 || id >= p.V) continue;
+        const bf16 *h = p.h + r * p.ldh, *w = p.w + id * p.ldw;
+        float sum[8] = {};
+#pragma unroll 4
+        for (int k = lane * 8; k < p.K; k += 256) {
+          float a[8], b[8];
+          load_f32<8>(h + k, a);
+          load_f32<8>(w + k, b);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] = fmaf(a[i], b[i], sum[i]);
+        }
+        const float x = warp_sum(((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])));
+        if (lane == 0) p.summed[r] = x;
+      }
+      if (!mbar_wait_warp(tfull_bar(acc), (t >> 1) & 1, abort_flag)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + acc * kHeadCols + ((uint32_t)(q * 32) << 16);
+      const int width = min(p.V - n0, p.cols);
+      // the accumulator is free once its last columns are in registers: before the tally is stored, which the arrival would wait for
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_remote(leader_tempty + 8u * acc);
+          else mbar_arrive(tempty_bar(acc));
+        }
+      };
+      if (row0 >= p.T || half * 32 >= width) release();
       if (row0 < p.T) {
         PairTally run = pair_empty();
-        for (int c0 = 0; c0 < p.cols; c0 += 32) {
+        for (int c0 = half * 32; c0 < width; c0 += 64) {
           uint32_t r[32];
           tmem_ld32(taddr + c0, r);
           tmem_ld_wait();
-          const int left = p.V - n0 - c0;
+          if (c0 + 64 >= width) release();
+          const int left = min(32, width - c0);
           if (left < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (j >= left) r[j] = 0xFF800000u;
           }
-          float most = __uint_as_float(r[0]);
+          float most[4];
 #pragma unroll
-          for (int j = 1; j < 32; ++j) most = fmaxf(most, __uint_as_float(r[j]));
-          if (most > run.m) pair_rebase(run, most, c);
+          for (int i = 0; i < 4; ++i) {
+            most[i] = __uint_as_float(r[i]);
+#pragma unroll
+            for (int j = i + 4; j < 32; j += 4) most[i] = fmaxf(most[i], __uint_as_float(r[j]));
+          }
+          most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+          if (most[0] > run.m) pair_rebase(run, most[0], c);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) pair_add(run, {__uint_as_float(r[j]), __uint_as_float(r[j + 1])}, c);
-          const bool here = want >= c0 && want < c0 + 32 && want < p.V - n0;
+          const bool here = want >= c0 && want < c0 + left;
           if (__any_sync(0xffffffffu, here)) {
             float x = 0.f;
 #pragma unroll
@@ -186,56 +300,88 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
             if (here) p.given[row] = x;
           }
         }
-        if (row < p.T) p.tallies[(int64_t)n * p.T + row] = pair_sum(run);
+        // the row's other thread: a barrier for the two warps, and one more before its place is written again
+        Tally a = pair_sum(run);
+        Tally* other = reinterpret_cast<Tally*>(smem + kHeadRing + kHeadFixed) + q * 32 + lane;
+        if (half == 1) *other = a;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        if (half == 0) {
+          a = tally_join(a, *other, c);
+          if (row < p.T) p.tallies[(int64_t)row * p.n_tiles + n] = make_float4(a.m, a.z, a.s, 0.f);
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(leader_tempty + 8u * acc);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_head_error, 1);
-  cluster_sync();                                     // neither CTA leaves while the other may touch its barriers or memory
+  if constexpr (PAIR) cluster_sync();                 // neither CTA leaves while the other may touch its barriers or memory
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
   }
 }
 
-// A block joins `rows` rows (a power of two, 32 at most), 256 / rows threads each: a thread every so many tiles, then in pairs.
-__global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int rows, float* out_lp, float* out_entropy) {
-  __shared__ Tally part[256];
+// `threads` of a block (a warp, or all of them) join a row: a thread every so many tiles, then in pairs.
+__global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int threads, float* out_lp, float* out_entropy) {
+  __shared__ Tally part[8];
   pdl_wait();
-  const int r = threadIdx.x % rows, slice = threadIdx.x / rows, slices = 256 / rows;
-  const int64_t row = (int64_t)blockIdx.x * rows + r;
+  const int t = threadIdx.x % threads, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * (256 / threads) + threadIdx.x / threads;
+  if (row >= p.T) return;                            // whole warps; no block is left by some of the threads of a row
+  const float scale = row_scale(p.temperature, row), c = scale * kLog2e;
+  const int64_t id = p.ids[row];
+  const bool given = id >= 0 && id < p.V;
+  const float x0 = given ? p.given[row] : 0.f, x = given ? p.summed[row] : 0.f;
+  const float4* tallies = p.tallies + row * p.n_tiles;
   Tally a = tally_empty();
-  float scale = 1.f, c = kLog2e;
-  if (row < p.T) {
-    scale = row_scale(p.temperature, row);
-    c = scale * kLog2e;
-    for (int i = slice; i < p.n_tiles; i += slices) a = tally_join(a, p.tallies[(int64_t)i * p.T + row], c);
+  for (int i = t; i < p.n_tiles; i += 4 * threads) {
+    Tally b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      b[j] = tally_empty();
+      if (i + j * threads < p.n_tiles) {
+        const float4 v = tallies[i + j * threads];
+        b[j] = {v.x, v.y, v.z};
+      }
+    }
+    a = tally_join(a, tally_join(tally_join(b[0], b[1], c), tally_join(b[2], b[3], c), c), c);
   }
-  part[threadIdx.x] = a;
-  __syncthreads();
-  for (int half = slices / 2; half > 0; half /= 2) {
-    if (slice < half) part[threadIdx.x] = a = tally_join(a, part[threadIdx.x + half * rows], c);
+  tally_rebase(a, warp_max(a.m), c);
+  a.z = warp_sum(a.z);
+  a.s = warp_sum(a.s);
+  if (threads > 32) {
+    if (lane == 0) part[wid] = a;
     __syncthreads();
+    a = part[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) a = tally_join(a, part[w], c);
   }
-  if (slice == 0 && row < p.T) {
-    const int64_t id = p.ids[row];
-    out_lp[row] = id < 0 ? 0.f : id >= p.V ? -INFINITY : tally_logprob(a, p.given[row], scale);
-    out_entropy[row] = tally_entropy(a);
+  if (t != 0) return;
+  float lp = id < 0 ? 0.f : -INFINITY;
+  if (given) {
+    // the given token's term as it was tallied makes way for the one of its rounded sum
+    const float t0 = bounded((x0 - a.m) * c), t1 = bounded((x - a.m) * c), e0 = exp2_fast(t0), e1 = exp2_fast(t1);
+    a.z += e1 - e0;
+    a.s += e1 * t1 - e0 * t0;
+    lp = tally_logprob(a, x, scale);
   }
+  out_lp[row] = lp;
+  out_entropy[row] = tally_entropy(a);
 }
 
-// Columns of a tile: the width whose rounds over the 74 pairs of SMs cost least, a round as its columns and some 32 for its ends.
-static int head_cols(int rows, int vocab) {
-  const int64_t m_tiles = (rows + 2 * kHeadRows - 1) / (2 * kHeadRows);
-  int64_t best = 0;
+// Columns of a tile: the width whose rounds over the SMs (or pairs of them) and last tally cost least.  A round costs its columns and
+// some 16 (a pair's some 32) for its ends; a tally 16 ns a column, where loading a column takes an SM 0.045 ns K.
+static int head_cols(int rows, int vocab, int width) {
+  const bool pair = rows > kHeadRows;
+  const int64_t m_tiles = (rows + 2 * kHeadRows - 1) / (2 * kHeadRows), slots = pair ? 74 : 148;
+  double best = 0;
   int cols = kHeadCols;
-  for (int c = kHeadCols; c >= 128; c -= 32) {
-    const int64_t tiles = m_tiles * ((vocab + c - 1) / c), cost = (tiles + 73) / 74 * (c + 32);
+  for (int c = kHeadCols; c >= 128; c -= 16) {
+    const int64_t tiles = m_tiles * ((vocab + c - 1) / c);
+    const double cost = (double)((tiles + slots - 1) / slots) * (c + (pair ? 32 : 16)) + c * 350. / width;
     if (best == 0 || cost < best) {
       best = cost;
       cols = c;
@@ -244,13 +390,39 @@ static int head_cols(int rows, int vocab) {
   return cols;
 }
 
+template <bool PAIR>
+static cudaError_t launch_head_tally(const CUtensorMap& h, const CUtensorMap& w, const HeadParams& p, int ctas, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool attr_done[64] = {};
+  if (!attr_done[dev & 63]) {
+    const cudaError_t e = cudaFuncSetAttribute(head_tally_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem);
+    if (e != cudaSuccess) return e;
+    attr_done[dev & 63] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kHeadThreads);
+  cfg.dynamicSmemBytes = kHeadSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, head_tally_kernel<PAIR>, h, w, p);
+}
+
 }  // namespace xllm
 
 // Bytes of workspace of xllm_head_logprobs.
-XLLM_API int64_t xllm_head_logprobs_workspace(int rows, int vocab) {
+XLLM_API int64_t xllm_head_logprobs_workspace(int rows, int vocab, int width) {
   using namespace xllm;
-  const int cols = head_cols(rows, vocab);
-  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(Tally) + sizeof(float)) * rows;
+  const int cols = head_cols(rows, vocab, width);
+  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(float4) + 2 * sizeof(float)) * rows;
 }
 
 // Reads and clears the error word: non-zero when a bounded wait expired since the last query.
@@ -272,29 +444,31 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   if (rows == 0) return 0;
   if (rows < 0 || vocab < 1 || width < 1 || width % 8 || ldh % 8 || ldw % 8) return (int)cudaErrorInvalidValue;
   if (((uintptr_t)hidden | (uintptr_t)weight) & 15) return (int)cudaErrorInvalidValue;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  static bool attr_done[64] = {};
-  if (!attr_done[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(head_tally_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem);
-    if (e != cudaSuccess) return (int)e;
-    attr_done[dev & 63] = true;
-  }
-  const int cols = head_cols(rows, vocab), n_tiles = (vocab + cols - 1) / cols;
+  const bool pair = rows > kHeadRows;
+  const int cols = head_cols(rows, vocab, width), n_tiles = (vocab + cols - 1) / cols, w_box = pair ? cols / 2 : cols;
   const int m_tiles = (rows + 2 * kHeadRows - 1) / (2 * kHeadRows), a_box = rows >= kHeadRows ? kHeadRows : (rows + 7) & ~7;
-  if ((int64_t)m_tiles * n_tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
+  if ((int64_t)m_tiles * n_tiles > 0x3fffffff) return (int)cudaErrorInvalidValue;
   CUtensorMap map_h, map_w;
-  if (!make_map(&map_h, hidden, rows, width, ldh, a_box) || !make_map(&map_w, weight, vocab, width, ldw, cols / 2))
+  if (!make_map(&map_h, hidden, rows, width, ldh, a_box) || !make_map(&map_w, weight, vocab, width, ldw, w_box))
     return (int)cudaErrorInvalidValue;
-  Tally* tallies = (Tally*)workspace;
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, (const int64_t*)ids, (const float*)temperature, tallies,
-                     (float*)(tallies + (int64_t)n_tiles * rows)};
+  // a stage costs the issuing warps some 370 cycles whatever it holds: two K blocks where they are small (64 x 1024 x 32768: 17.5 us,
+  // 19.0 with one; 128 rows in tiles of 208 columns, 4096 x 151936: 211 us, 199 with one)
+  const int per_stage = a_box + w_box <= 192 ? 2 : 1;
+  // the products read 128 rows of h of which a_box are loaded: the last stage's lie in front of the ring's end as well
+  const int stage_bytes = per_stage * (a_box + w_box) * kHeadK * 2, slack = (kHeadRows - a_box) * kHeadK * 2;
+  int stages = (kHeadRing - slack) / stage_bytes;
+  if (stages > kHeadMostStages) stages = kHeadMostStages;
+  float4* tallies = (float4*)workspace;
+  float* given = (float*)(tallies + (int64_t)n_tiles * rows);
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, (const bf16*)hidden, ldh,
+                     (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows};
   cudaStream_t s = (cudaStream_t)stream;
-  const int pairs = m_tiles * n_tiles < 74 ? m_tiles * n_tiles : 74;
-  cudaError_t e = launch_pdl(head_tally_kernel, dim3(2 * pairs), dim3(kHeadThreads), kHeadSmem, s, map_h, map_w, p);
+  const int units = m_tiles * n_tiles;
+  cudaError_t e = pair ? launch_head_tally<true>(map_h, map_w, p, 2 * (units < 74 ? units : 74), s)
+                       : launch_head_tally<false>(map_h, map_w, p, units, s);
   if (e != cudaSuccess) return (int)e;
-  int join = 1;
-  while (join < 32 && join < rows) join *= 2;
-  e = launch_pdl(head_join_kernel, dim3((rows + join - 1) / join), dim3(256), 0, s, p, join, (float*)out_lp, (float*)out_entropy);
+  const int threads = rows <= 296 ? 256 : 32;
+  e = launch_pdl(head_join_kernel, dim3((unsigned)(((int64_t)rows * threads + 255) / 256)), dim3(256), 0, s, p, threads, (float*)out_lp,
+                 (float*)out_entropy);
   return e != cudaSuccess ? (int)e : XLLM_LAUNCH_CHECK();
 }

@@ -195,6 +195,25 @@ __host__ __device__ constexpr uint32_t idesc_pair(int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 }
 
+// ------------------------------------------------------------------------ work handed out by the hardware
+// A running CTA takes over one that has not started (a grid of single CTAs): the answer, 16 bytes, arrives at `dst` and counts on
+// `bar`.  After a refusal nothing more is asked for.
+__device__ __forceinline__ void take_cta(uint32_t dst, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ int taken_cta(uint32_t src) {        // its index, or -1
+  int x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 answer;\n\tld.shared.b128 answer, [%1];\n\tmov.s32 %0, -1;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, answer;\n\t}"
+      : "=r"(x)
+      : "r"(src)
+      : "memory");
+  return x;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

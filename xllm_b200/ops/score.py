@@ -18,7 +18,7 @@ from ._lib import I, L, P, check, ptr, stream_on
 
 _lib.register_signature("xllm_token_logprobs", [P, L, I, I, I, P, P, I, P, P, P, P, P])
 _lib.register_signature("xllm_head_logprobs", [P, L, P, L, I, I, I, P, P, P, P, P, P])
-_lib.register_signature("xllm_head_logprobs_workspace", [I, I], L)
+_lib.register_signature("xllm_head_logprobs_workspace", [I, I, I], L)
 _lib.register_signature("xllm_head_logprobs_error_status", [], I)
 
 MAX_TOP = 128          # alternatives a row can list
@@ -150,7 +150,7 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     lib = _lib.load()
     lp = torch.empty(rows, dtype=torch.float32, device=dev)
     entropy = torch.empty_like(lp)
-    work = torch.empty(lib.xllm_head_logprobs_workspace(rows, vocab), dtype=torch.uint8, device=dev)
+    work = torch.empty(lib.xllm_head_logprobs_workspace(rows, vocab, width), dtype=torch.uint8, device=dev)
     check(lib.xllm_head_logprobs(ptr(hidden), _stride(hidden), ptr(weight), _stride(weight), rows, vocab, width, ptr(ids),
                                  ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream_on(index)), "head_logprobs")
     _count(2)
