@@ -40,6 +40,10 @@ def call(llm: LLM, method: str, args_json: str) -> str:
         outs = llm.embed(a["prompts"])
         return json.dumps([[float(x) for x in o.outputs.embedding] if hasattr(o, "outputs") else [float(x) for x in o]
                            for o in outs])
+    if method == "score":
+        outs = llm.score(a["prompts"], top_logprobs=int(a.get("top_logprobs", 0)), temperature=a.get("temperature"))
+        return json.dumps([{"token_ids": o.prompt_token_ids, "logprobs": o.logprobs, "entropies": o.entropies,
+                            "top_logprobs": o.top_logprobs} for o in outs])
     if method == "beam_search":
         res = llm.beam_search(a["prompt"], beam_width=int(a.get("beam_width", 4)), max_tokens=int(a.get("max_tokens", 16)),
                               ignore_eos=bool(a.get("ignore_eos", False)))[0]     # one prompt -> its beams

@@ -107,6 +107,22 @@ class EmbeddingOutput:
     status: Optional[object] = None
 
 
+@dataclass
+class ScoreOutput:
+    """Result of `LLM.score` for one prompt, an entry per token: its log-probability given the tokens before it, the entropy of
+    the distribution it was picked from and, where asked for, that distribution's most likely tokens.  None for the first one."""
+    prompt: Optional[str]
+    prompt_token_ids: List[int]
+    logprobs: List[Optional[float]]
+    entropies: List[Optional[float]]
+    top_logprobs: Optional[List[Optional[List[tuple]]]] = None
+    usage: Usage = field(default_factory=Usage)
+
+    @property
+    def total_logprob(self) -> float:
+        return sum(v for v in self.logprobs if v is not None)
+
+
 class LLM:
     """Offline batch inference over one engine (single GPU, or one rank of a TP job)."""
 
@@ -372,6 +388,17 @@ class LLM:
                     ro.outputs.append(so)
             outs.append(ro)
         return outs
+
+    def score(self, prompts, top_logprobs: int = 0, temperature: Optional[float] = None) -> List[ScoreOutput]:
+        """Log-probability of every token of every prompt under softmax(logits / temperature), with its distribution's entropy and
+        `top_logprobs` alternatives; nothing is generated.  Prompts are strings or token ids; short ones share passes."""
+        from .scoring import score_token_lists
+        if isinstance(prompts, (str, torch.Tensor)) or (prompts and isinstance(prompts[0], int)):
+            prompts = [prompts]
+        ids = [self._encode(p) for p in prompts]
+        scores = score_token_lists(self.engine, ids, top_logprobs, temperature)
+        return [ScoreOutput(p if isinstance(p, str) else None, i, s.logprobs, s.entropies, s.top_logprobs, Usage(len(i), 0, len(i), 0))
+                for p, i, s in zip(prompts, ids, scores)]
 
     def sleep(self, level: int = 1):
         """Release the KV cache (level 1) and also move the weights to host memory (level 2)."""

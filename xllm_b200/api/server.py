@@ -2,7 +2,7 @@
 
 Route parity with the reference's APIService / XllmServer (xllm/server/xllm_server.cpp:39-60,
 xllm/api_service/*): `/v1/completions`, `/v1/chat/completions` (SSE streaming and plain),
-`/v1/models`, `/v1/embeddings`, `/v1/messages` (Anthropic), `/health`, `/metrics` and the admin
+`/v1/models`, `/v1/embeddings`, `/v1/score`, `/v1/messages` (Anthropic), `/health`, `/metrics` and the admin
 endpoints `/sleep`, `/wakeup`, `/pause`, `/resume`, `/start_profile`, `/stop_profile`.
 Tool-call and reasoning parsing of chat responses uses the C++ stream parsers; request ids,
 `max_concurrent_requests` rate limiting and client-disconnect aborts follow
@@ -291,7 +291,7 @@ class ApiServer:
                 return self._error(req.id, 400, f"invalid JSON body: {e}")
         # another model served by this process (fork_master): same routes, its own engine
         target = self.forks.get(str(body.get("model") or body.get("model_id") or ""))
-        if target is not None and path in self.GENERATION_PATHS + ("/v1/embeddings", "/v1/rerank", "/v1/sample",
+        if target is not None and path in self.GENERATION_PATHS + ("/v1/embeddings", "/v1/rerank", "/v1/sample", "/v1/score",
                                                                    "/sleep", "/wakeup", "/pause", "/resume"):
             return target._route(req, prepared)
         if path == "/v1/completions":
@@ -312,6 +312,8 @@ class ApiServer:
             return self._rerank(req, body)
         if path == "/v1/sample":
             return self._sample(req, body)
+        if path == "/v1/score":
+            return self._score(req, body)
         if path == "/v1/images/generations":
             return self._images(req, body)
         if path == "/pause":
@@ -749,6 +751,29 @@ class ApiServer:
                                  "usage": {"prompt_tokens": len(ids), "total_tokens": len(ids)}})
 
     # ------------------------------------------------------------------ output events
+    def _score(self, req, body):
+        """Log-probabilities of the prompts' own tokens: `prompt` (text, token ids, or a list of either), `logprobs` alternatives."""
+        from .scoring import score_token_lists
+        prompts = body.get("prompt")
+        if isinstance(prompts, str) or (isinstance(prompts, list) and prompts and isinstance(prompts[0], int)):
+            prompts = [prompts]
+        if not isinstance(prompts, list) or not prompts or not all(isinstance(p, (str, list)) for p in prompts):
+            return self._error(req.id, 400, "prompt must be a text, token ids, or a list of either")
+        try:
+            ids = [self.tok.encode(p) if isinstance(p, str) else [int(t) for t in p] for p in prompts]
+            n_top, t = int(body.get("logprobs") or 0), body.get("temperature")
+            scores = score_token_lists(self.engine, ids, n_top, None if t is None else float(t))
+        except (TypeError, ValueError) as e:
+            return self._error(req.id, 400, str(e))
+        choices = [{"index": k, "logprobs": {"tokens": [self.tok.decode([t]) for t in i], "token_ids": i, "token_logprobs": s.logprobs,
+                                             "entropies": s.entropies,
+                                             "top_logprobs": None if s.top_logprobs is None else
+                                             [None if a is None else [{"token_id": t, "logprob": v} for t, v in a] for a in s.top_logprobs]}}
+                   for k, (i, s) in enumerate(zip(ids, scores))]
+        n = sum(map(len, ids))
+        self._json(req.id, 200, {"id": body.get("request_id") or "score-" + str(req.id), "object": "score", "created": int(time.time()),
+                                 "model": self.model_name, "choices": choices, "usage": {"prompt_tokens": n, "total_tokens": n}})
+
     def _sse(self, call, obj):
         self.http.stream_send(call.http_id, "data: " + json.dumps(obj, ensure_ascii=False) + "\n\n")
 
