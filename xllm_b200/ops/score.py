@@ -55,16 +55,16 @@ def token_logprobs_reference(logits, ids, n_top=0, temperature=None):
 
 
 def _check_rows(x, ids, temperature, name):
-    """Refuses what no kernel reads; returns the rows' device."""
+    """Refuses what no kernel reads; returns (rows, columns, device)."""
     dev = x.device
     if x.dim() != 2 or x.stride(1) != 1 and x.shape[1] > 1:
         raise ValueError(f"{name}: rows [rows, columns] with adjacent columns expected, got {tuple(x.shape)} strides {x.stride()}")
-    rows = x.shape[:1]
-    if ids.dtype != torch.int64 or ids.shape != rows or ids.device != dev:
-        raise TypeError(f"{name}: ids are int64 [{x.shape[0]}] on {dev}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-    if temperature is not None and (temperature.dtype != torch.float32 or temperature.shape != rows or temperature.device != dev):
-        raise TypeError(f"{name}: temperatures are fp32 [{x.shape[0]}] on {dev}")
-    return dev
+    n, columns = x.shape
+    if ids.dtype is not torch.int64 or ids.shape != (n,) or ids.device != dev:
+        raise TypeError(f"{name}: ids are int64 [{n}] on {dev}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+    if temperature is not None and (temperature.dtype is not torch.float32 or temperature.shape != (n,) or temperature.device != dev):
+        raise TypeError(f"{name}: temperatures are fp32 [{n}] on {dev}")
+    return n, columns, dev
 
 
 def _dense(t):
@@ -76,18 +76,17 @@ def token_logprobs(logits, ids, n_top=0, temperature=None):
     [rows] or None.  Returns (logprob fp32 [rows], entropy fp32 [rows], alternatives int32 [rows, n_top], their
     log-probabilities fp32 [rows, n_top]); the alternatives are the n_top largest logits, largest first, ties to the lowest index, -1 and
     -inf where the row has no more tokens above -inf, and None without n_top."""
-    dev = _check_rows(logits, ids, temperature, "token_logprobs")
-    rows, vocab = logits.shape
+    rows, vocab, dev = _check_rows(logits, ids, temperature, "token_logprobs")
     if vocab < 1 or not 0 <= n_top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_logprobs: 0 to {min(MAX_TOP, vocab)} alternatives of a vocabulary of {vocab}, asked for {n_top}")
     if _debug.enabled():
         _debug.check_range(ids, 0, vocab, "token_logprobs ids", allow_negative_skip=True)
+    index = dev.index
     if not logits.is_cuda:
         return token_logprobs_reference(logits, ids, n_top, temperature)
-    dt = 0 if logits.dtype == torch.bfloat16 else 1
-    if dt == 1 and logits.dtype != torch.float32:
+    dt = 0 if logits.dtype is torch.bfloat16 else 1
+    if dt == 1 and logits.dtype is not torch.float32:
         logits = logits.float()
-    index = dev.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return token_logprobs(logits, ids, n_top, temperature)
@@ -96,8 +95,8 @@ def token_logprobs(logits, ids, n_top=0, temperature=None):
     entropy = torch.empty_like(lp)
     top = top_lp = None
     if n_top:
-        top = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
         top_lp = lp.new_empty((rows, n_top))
+        top = torch.empty_like(top_lp, dtype=torch.int32)
     check(_lib.load().xllm_token_logprobs(ptr(logits), logits.stride(0), dt, rows, vocab, ptr(ids), ptr(temperature), int(n_top),
                                           ptr(lp), ptr(entropy), ptr(top), ptr(top_lp), stream_on(index)), "token_logprobs")
     _count()
@@ -124,12 +123,11 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     and weight [vocab, width] bf16, the products' sums fp32 and never rounded to bf16 (so not the bits of the two steps, which
     round every logit).  Returns (logprob, entropy) fp32 [rows].  On CUDA the width is a multiple of 8 and rows start on
     16-byte boundaries."""
-    dev = _check_rows(hidden, ids, temperature, "head_logprobs")
+    rows, width, dev = _check_rows(hidden, ids, temperature, "head_logprobs")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.stride(-1) != 1 or weight.dtype != hidden.dtype \
             or weight.shape[0] < 1 or weight.device != hidden.device:
         raise ValueError(f"head_logprobs: weight [vocab, {hidden.shape[1]}] {hidden.dtype} on {hidden.device} expected, got "
                          f"{tuple(weight.shape)} {weight.dtype} on {weight.device}")
-    rows, width = hidden.shape
     vocab = weight.shape[0]
     if _debug.enabled():
         _debug.check_range(ids, 0, vocab, "head_logprobs ids", allow_negative_skip=True)

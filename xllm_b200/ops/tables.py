@@ -63,15 +63,15 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
     passes 31 bits, has slot -1.  Nothing is read back: whoever may run short compares kv_lens later.
 
     ctx_lens, q_lens: int32 [requests], negative ones count as 0.  Returns StepTables."""
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[1] > 1 and block_table.stride(1) != 1:
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
         raise TypeError(f"step_tables: block_table is int32 [requests, width] with adjacent entries, got {block_table.dtype} "
                         f"{tuple(block_table.shape)} strides {block_table.stride()}")
     B, width = block_table.shape
     dev = block_table.device
-    for t, name in ((ctx_lens, "ctx_lens"), (q_lens, "q_lens")):
-        if t.dtype != torch.int32 or t.shape != (B,) or t.device != dev:
-            raise TypeError(f"step_tables: {name} is int32 [{B}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if free_blocks is not None and (free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or free_blocks.device != dev):
+    if not (ctx_lens.dtype is q_lens.dtype is torch.int32 and ctx_lens.shape == q_lens.shape == (B,) and ctx_lens.device == q_lens.device == dev):
+        raise TypeError(f"step_tables: ctx_lens and q_lens are int32 [{B}] on {dev}, got {ctx_lens.dtype} {tuple(ctx_lens.shape)} on "
+                        f"{ctx_lens.device}, {q_lens.dtype} {tuple(q_lens.shape)} on {q_lens.device}")
+    if free_blocks is not None and (free_blocks.dtype is not torch.int32 or free_blocks.dim() != 1 or free_blocks.device != dev):
         raise TypeError(f"step_tables: free_blocks is int32 [blocks] on {dev}")
     if not 1 <= B <= MAX_REQUESTS or width < 1 or page < 1 or not 0 <= n_rows < 1 << 31:
         raise ValueError(f"step_tables: 1 to {MAX_REQUESTS} requests, a width and a page of 1 or more and 0 or more rows, got "
@@ -90,12 +90,14 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
     n_free = 0
     if free_blocks is not None:
         free_blocks, n_free = free_blocks.contiguous(), free_blocks.shape[0]
-    # one allocation for each type: half a step's time is the host's
-    cu_q, kv_lens, slots, taken = torch.empty(2 * B + n_rows + 2, dtype=torch.int32, device=dev).split_with_sizes([B + 1, B, n_rows, 1])
-    positions, last_rows = torch.empty(n_rows + B, dtype=torch.int64, device=dev).split_with_sizes([n_rows, B])
-    out = StepTables(cu_q, kv_lens, positions, slots, last_rows, taken.view(()))
+    # one allocation: a short step's time is the host's
+    i64 = 2 * (n_rows + B)
+    buf = torch.empty(i64 + n_rows + 2 * B + 2, dtype=torch.int32, device=dev)
+    positions, last_rows, slots, cu_q, kv_lens, taken = buf.split_with_sizes([2 * n_rows, 2 * B, n_rows, B + 1, B, 1])
+    at = buf.data_ptr()
+    rest = at + 4 * i64
     check(_lib.load().xllm_step_tables(ptr(block_table), block_table.stride(0), B, width, ptr(ctx_lens), ptr(q_lens), int(page),
-                                       int(n_rows), ptr(free_blocks), n_free, ptr(cu_q), ptr(kv_lens), ptr(positions), ptr(slots),
-                                       ptr(last_rows), ptr(taken), stream_on(index)), "step_tables")
+                                       int(n_rows), ptr(free_blocks), n_free, rest + 4 * n_rows, rest + 4 * (n_rows + B + 1), at, rest,
+                                       at + 8 * n_rows, rest + 4 * (n_rows + 2 * B + 1), stream_on(index)), "step_tables")
     _count()
-    return out
+    return StepTables(cu_q, kv_lens, positions.view(torch.int64), slots, last_rows.view(torch.int64), taken.view(()))
