@@ -171,6 +171,30 @@ def test_many_candidates(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_scores_and_small_temperatures(device, dtype):
+    """Scores of thousands, scores whose differences count in the 7th place, temperatures that leave one token, masks among them."""
+    g = torch.Generator().manual_seed(21)
+    V = 9000
+    x = torch.randn(8, V, generator=g) * 3
+    x[1] += 5000.0
+    x[2] -= 30000.0
+    x[3] *= 400.0
+    x[4] = 1000.0 + torch.rand(V, generator=g)
+    x[5, ::3] = -math.inf
+    x[6, 100:] = -math.inf
+    x[7, 50:8000] = torch.finfo(dtype).min
+    x = x.to(dtype).to(device)
+    ids = x.float().argmax(1)
+    ids[::2] = 11
+    compare(score.token_logprobs(x, ids, 3), x, ids, 3)
+    for t in (1e-3, 1e-5, 1e-8, 30.0, 1e5):
+        some = x[:7]
+        T = torch.full((7,), t, device=device)
+        compare(score.token_logprobs(some, ids[:7], 3, temperature=T), some, ids[:7], 3, T)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_strides_and_types(device):
     x, ids, t = rows(6, 500, torch.bfloat16, 2, device, 9)
     want = score.token_logprobs(x.contiguous(), ids, 4, temperature=t)
