@@ -220,19 +220,19 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
       id_next = row < p.T ? p.ids[row] : -1;
       c_next = row < p.T ? row_scale(p.temperature, row) * kLog2e : kLog2e;
     };
-    int t = 0, m, n;
+    int t = 0, m, n, m_next, n_next;
     bool ok = true;
-    head_tile(p, first, m, n);
-    fetch(m);
+    head_tile(p, first, m_next, n_next);
+    fetch(m_next);
     for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
-      head_tile(p, u, m, n);
+      m = m_next;
+      n = PAIR ? n_next : u;
       const int row0 = row_of(m), row = row0 + lane, n0 = n * p.cols, acc = t & 1;
       const float c = c_next;
       const int64_t want = id_next - n0;              // the given token's column, if it is one of this tile's
       if (PAIR && u + (int)(gridDim.x >> 1) < units) {
-        int m1, n1;
-        head_tile(p, u + (gridDim.x >> 1), m1, n1);
-        if (m1 != m) fetch(m1);
+        head_tile(p, u + (gridDim.x >> 1), m_next, n_next);
+        if (m_next != m) fetch(m_next);
       }
       // The tensor cores' sums of K products are cut off at every step, some 2^-19 of a large score in all.  While the tile is
       // computed, the given tokens' scores are summed once more as fp32 products that round: a warp a row, shared out by the tiles.
@@ -257,7 +257,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
       tc_fence_after();
       const uint32_t taddr = tmem_base + acc * kHeadCols + ((uint32_t)(q * 32) << 16);
       const int width = min(p.V - n0, p.cols);
-      // the accumulator is free once its last columns are in registers: before the tally is stored, which the arrival would wait for
+      // the accumulator is free once its last columns are in registers
       const auto release = [&] {
         tc_fence_before();
         __syncwarp();

@@ -44,26 +44,10 @@ __device__ __forceinline__ Tally tally_join(Tally a, Tally b, float c) {
   return {m, a.z + b.z, a.s + b.s};
 }
 // Pairs of fp32 in one instruction.
-struct f32x2 {
-  float x, y;
-};
-#define XLLM_F32X2(name, op)                                                                                         \
-  __device__ __forceinline__ f32x2 name(f32x2 a, f32x2 b) {                                                          \
-    f32x2 r;                                                                                                         \
-    asm("{\n\t.reg .b64 p, q, s;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\t" op                             \
-        " s, p, q;\n\tmov.b64 {%0, %1}, s;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));   \
-    return r;                                                                                                        \
-  }
-XLLM_F32X2(add2, "add.rn.f32x2")
-XLLM_F32X2(mul2, "mul.rn.f32x2")
-#undef XLLM_F32X2
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("{\n\t.reg .b64 p, q, s, t;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 s, {%6, %7};\n\t"
-      "fma.rn.f32x2 t, p, q, s;\n\tmov.b64 {%0, %1}, t;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
+typedef float2 f32x2;
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __ffma2_rn(a, b, c); }
 
 // A tally that takes two scores at a time: its sums are those of the first and of the second ones.
 struct PairTally {
