@@ -467,7 +467,7 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   cudaError_t e = pair ? launch_head_tally<true>(map_h, map_w, p, 2 * (units < 74 ? units : 74), s)
                        : launch_head_tally<false>(map_h, map_w, p, units, s);
   if (e != cudaSuccess) return (int)e;
-  const int threads = rows <= 296 ? 256 : 32;
+  const int threads = rows <= 296 && n_tiles > 128 ? 256 : 32;       // a block a row while that fills the SMs
   e = launch_pdl(head_join_kernel, dim3((unsigned)(((int64_t)rows * threads + 255) / 256)), dim3(256), 0, s, p, threads, (float*)out_lp,
                  (float*)out_entropy);
   return e != cudaSuccess ? (int)e : XLLM_LAUNCH_CHECK();

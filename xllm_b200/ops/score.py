@@ -11,6 +11,8 @@ Sums, maxima and results are fp32 whatever the scores' type.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _count, _debug, _lib
@@ -118,10 +120,16 @@ def head_supported(hidden, weight):
             and not (_stride(hidden) | _stride(weight)) % 8 and not (hidden.data_ptr() | weight.data_ptr()) % 16)
 
 
+@functools.lru_cache(maxsize=4096)
+def _head_workspace(rows, vocab, width):
+    return _lib.load().xllm_head_logprobs_workspace(rows, vocab, width)
+
+
 def head_logprobs(hidden, weight, ids, temperature=None):
     """The log-probabilities and entropies of token_logprobs(hidden @ weight^T, ids) without the logits: hidden [rows, width]
     and weight [vocab, width] bf16, the products' sums fp32 and never rounded to bf16 (so not the bits of the two steps, which
-    round every logit).  Returns (logprob, entropy) fp32 [rows].  On CUDA the width is a multiple of 8 and rows start on
+    round every logit).  Returns (logprob, entropy) fp32 [rows].  A workspace of 16 bytes for each row and up to 256 tokens of
+    the vocabulary is allocated.  On CUDA the width is a multiple of 8 and rows start on
     16-byte boundaries."""
     rows, width, dev = _check_rows(hidden, ids, temperature, "head_logprobs")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.stride(-1) != 1 or weight.dtype != hidden.dtype \
@@ -145,11 +153,10 @@ def head_logprobs(hidden, weight, ids, temperature=None):
         hidden = hidden.contiguous()
     if _stride(weight) < width:
         weight = weight.contiguous()
-    lib = _lib.load()
     lp = torch.empty(rows, dtype=torch.float32, device=dev)
     entropy = torch.empty_like(lp)
-    work = torch.empty(lib.xllm_head_logprobs_workspace(rows, vocab, width), dtype=torch.uint8, device=dev)
-    check(lib.xllm_head_logprobs(ptr(hidden), _stride(hidden), ptr(weight), _stride(weight), rows, vocab, width, ptr(ids),
+    work = torch.empty(_head_workspace(rows, vocab, width), dtype=torch.uint8, device=dev)
+    check(_lib.load().xllm_head_logprobs(ptr(hidden), _stride(hidden), ptr(weight), _stride(weight), rows, vocab, width, ptr(ids),
                                  ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream_on(index)), "head_logprobs")
     _count(2)
     return lp, entropy
