@@ -241,6 +241,8 @@ def test_refusals():
     with pytest.raises(TypeError):
         score.token_logprobs(x, ids.int())
     with pytest.raises(TypeError):
+        score.token_logprobs(x.long(), ids)
+    with pytest.raises(TypeError):
         score.token_logprobs(x, ids[:3])
     with pytest.raises(TypeError):
         score.token_logprobs(x, ids, temperature=torch.ones(3))

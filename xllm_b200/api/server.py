@@ -759,8 +759,10 @@ class ApiServer:
             prompts = [prompts]
         if not isinstance(prompts, list) or not prompts or not all(isinstance(p, (str, list)) for p in prompts):
             return self._error(req.id, 400, "prompt must be a text, token ids, or a list of either")
+        if not all(isinstance(p, str) or all(isinstance(t, int) for t in p) for p in prompts):
+            return self._error(req.id, 400, "token ids are whole numbers")
         try:
-            ids = [self.tok.encode(p) if isinstance(p, str) else [int(t) for t in p] for p in prompts]
+            ids = [self.tok.encode(p) if isinstance(p, str) else p for p in prompts]
             n_top, t = int(body.get("logprobs") or 0), body.get("temperature")
             scores = score_token_lists(self.engine, ids, n_top, None if t is None else float(t))
         except (TypeError, ValueError) as e:

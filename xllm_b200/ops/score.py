@@ -74,21 +74,24 @@ def _dense(t):
 
 
 def token_logprobs(logits, ids, n_top=0, temperature=None):
-    """logits [rows, vocab] (bf16 or fp32; others are widened to fp32), rows at any stride; ids int64 [rows]; temperature fp32
+    """logits [rows, vocab] (bf16 or fp32; other floating types are converted to fp32), rows at any stride; ids int64 [rows]; temperature fp32
     [rows] or None.  Returns (logprob fp32 [rows], entropy fp32 [rows], alternatives int32 [rows, n_top], their
     log-probabilities fp32 [rows, n_top]); the alternatives are the n_top largest logits, largest first, ties to the lowest index, -1 and
-    -inf where the row has no more tokens above -inf, and None without n_top."""
+    -inf where the row has no more tokens above -inf, and None without n_top.  The sums' order, and with it a result's last bits, depends
+    on how many rows there are and how they lie in memory."""
     rows, vocab, dev = _check_rows(logits, ids, temperature, "token_logprobs")
     if vocab < 1 or not 0 <= n_top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_logprobs: 0 to {min(MAX_TOP, vocab)} alternatives of a vocabulary of {vocab}, asked for {n_top}")
     if _debug.enabled():
         _debug.check_range(ids, 0, vocab, "token_logprobs ids", allow_negative_skip=True)
     index = dev.index
-    if not logits.is_cuda:
-        return token_logprobs_reference(logits, ids, n_top, temperature)
     dt = 0 if logits.dtype is torch.bfloat16 else 1
     if dt == 1 and logits.dtype is not torch.float32:
+        if not logits.is_floating_point():
+            raise TypeError(f"token_logprobs: floating-point logits expected, got {logits.dtype}")
         logits = logits.float()
+    if not logits.is_cuda:
+        return token_logprobs_reference(logits, ids, n_top, temperature)
     if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return token_logprobs(logits, ids, n_top, temperature)

@@ -73,6 +73,8 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
                         f"{ctx_lens.device}, {q_lens.dtype} {tuple(q_lens.shape)} on {q_lens.device}")
     if free_blocks is not None and (free_blocks.dtype is not torch.int32 or free_blocks.dim() != 1 or free_blocks.device != dev):
         raise TypeError(f"step_tables: free_blocks is int32 [blocks] on {dev}")
+    if block_table.stride(0) < width and B > 1:
+        raise ValueError(f"step_tables: rows of block_table that lie apart, got strides {block_table.stride()} for {width} entries")
     if not 1 <= B <= MAX_REQUESTS or width < 1 or page < 1 or not 0 <= n_rows < 1 << 31:
         raise ValueError(f"step_tables: 1 to {MAX_REQUESTS} requests, a width and a page of 1 or more and 0 or more rows, got "
                          f"{B}, {width}, {page}, {n_rows}")
@@ -92,7 +94,7 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
         free_blocks, n_free = free_blocks.contiguous(), free_blocks.shape[0]
     # one allocation: a short step's time is the host's
     i64 = 2 * (n_rows + B)
-    buf = torch.empty(i64 + n_rows + 2 * B + 2, dtype=torch.int32, device=dev)
+    buf = ctx_lens.new_empty(i64 + n_rows + 2 * B + 2)
     positions, last_rows, slots, cu_q, kv_lens, taken = buf.split_with_sizes([2 * n_rows, 2 * B, n_rows, B + 1, B, 1])
     at = buf.data_ptr()
     rest = at + 4 * i64
