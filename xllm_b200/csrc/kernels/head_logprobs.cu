@@ -36,6 +36,7 @@ __device__ int g_head_error = 0;
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
   int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
+  int zeros;                                          // the others are zeros
   const bf16* h;
   int64_t ldh;
   const bf16* w;
@@ -76,7 +77,8 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
   const int units = p.m_tiles * p.n_tiles, k_blocks = (p.K + kHeadK - 1) / kHeadK;
   const int w_rows = PAIR ? p.cols / 2 : p.cols;                                  // of W that this CTA loads for a tile
-  const int a_bytes = p.a_box * kHeadK * 2, block_bytes = a_bytes + w_rows * kHeadK * 2;       // of a K block
+  constexpr int a_bytes = kHeadRows * kHeadK * 2;
+  const int block_bytes = a_bytes + w_rows * kHeadK * 2, loaded = block_bytes - (kHeadRows - p.a_box) * kHeadK * 2;       // of a K block
   const int stage_bytes = p.per_stage * block_bytes;
 
   if (threadIdx.x == 0) {
@@ -92,6 +94,16 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // Rows of h that are not there are zeros: what else lies in shared memory would be multiplied all the same, and draw power that the
+  // memory needs (one row x 4096 x 151936, sustained: 201 us at 1.4 GHz, 214 us at 0.86 GHz without).  Not where a call is too short
+  // for that to count, but not for the writing (64 x 512 x 32003: 15.3 us, 14.6 without).
+  if (p.zeros) {
+    const int vecs = (kHeadRows - p.a_box) * 8, blocks = p.stages * p.per_stage;
+    uint4* at = reinterpret_cast<uint4*>(smem + p.a_box * kHeadK * 2) + threadIdx.x;
+    for (int b = 0; b < blocks; ++b, at += block_bytes / 16)
+      for (int i = threadIdx.x; i < vecs; i += kHeadThreads) at[i - threadIdx.x] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
     if constexpr (PAIR) {
@@ -147,7 +159,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
         if (!mbar_wait_warp(empty_bar(stage), phase ^ 1, abort_flag)) { ok = false; break; }
         const int blocks = min(p.per_stage, k_blocks - kb);
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(full_bar(stage), (PAIR ? 2u : 1u) * blocks * block_bytes);
+          if (rank == 0) mbar_expect_tx(full_bar(stage), (PAIR ? 2u : 1u) * blocks * loaded);
           for (int i = 0; i < blocks; ++i) {
             const uint32_t dst = sbase + stage * stage_bytes + i * block_bytes;
             if constexpr (PAIR) {
@@ -454,13 +466,12 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   // a stage costs the issuing warps some 370 cycles whatever it holds: two K blocks where they are small (64 x 1024 x 32768: 17.5 us,
   // 19.0 with one; 128 rows in tiles of 208 columns, 4096 x 151936: 211 us, 199 with one)
   const int per_stage = a_box + w_box <= 192 ? 2 : 1;
-  // the products read 128 rows of h of which a_box are loaded: the last stage's lie in front of the ring's end as well
-  const int stage_bytes = per_stage * (a_box + w_box) * kHeadK * 2, slack = (kHeadRows - a_box) * kHeadK * 2;
-  int stages = (kHeadRing - slack) / stage_bytes;
+  int stages = kHeadRing / (per_stage * (kHeadRows + w_box) * kHeadK * 2);
   if (stages > kHeadMostStages) stages = kHeadMostStages;
   float4* tallies = (float4*)workspace;
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, (const bf16*)hidden, ldh,
+  const int zeros = a_box < kHeadRows && (int64_t)vocab * width > (64 << 20);
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, zeros, (const bf16*)hidden, ldh,
                      (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;
