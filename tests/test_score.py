@@ -405,6 +405,39 @@ def test_captured():
 
 
 @pytest.mark.gpu
+def test_captured_first_calls():
+    """A process whose first calls are captured ones."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from xllm_b200.ops import score, tables
+x, ids = torch.randn(9, 3000, device="cuda").bfloat16(), torch.arange(9, device="cuda")
+h, w = torch.randn(9, 64, device="cuda").bfloat16(), torch.randn(3000, 64, device="cuda").bfloat16()
+many = torch.randn(300, 64, device="cuda").bfloat16()
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+table, ctx, new, free = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), i32(3, 0), i32(2, 5), i32(7, 8, 9)
+calls = [lambda: score.token_logprobs(x, ids, 4), lambda: score.head_logprobs(h, w, ids),
+         lambda: score.head_logprobs(many, w, ids.repeat(34)[:300]), lambda: tables.step_tables(table, ctx, new, 4, 9, free)]
+torch.cuda.synchronize()
+graphs = []
+for f in calls:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = f()
+    graphs.append((g, out))
+for g, _ in graphs:
+    g.replay()
+torch.cuda.synchronize()
+for (_, out), f in zip(graphs, calls):
+    assert all(torch.equal(a, b) for a, b in zip(out, f()))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_rows_beyond_32_bits():
     """Row offsets that pass 2^31 elements."""
     V = 151936
