@@ -316,7 +316,7 @@ def test_head(device, T, K, V):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,K,V", [(1, 4096, 151936), (16, 512, 50257), (32, 2048, 32000), (45, 1024, 129280), (100, 512, 32003), (130, 512, 32768),
+@pytest.mark.parametrize("T,K,V", [(1, 4096, 151936), (16, 512, 50257), (17, 264, 30000), (63, 512, 20000), (65, 512, 20000), (32, 2048, 32000), (45, 1024, 129280), (100, 512, 32003), (130, 512, 32768),
                                    (300, 2880, 9000), (1000, 256, 40000), (4097, 128, 12345), (129, 2048, 3001), (200, 1024, 20000), (256, 1208, 5000)])
 def test_head_sizes(T, K, V):
     h, w, ids, t = head_case(T, K, V, 7, "cuda")

@@ -9,7 +9,8 @@
 // a ring of stages, one thread of the pair's first CTA issues the products into one of two accumulators in tensor memory, and eight
 // warps of each CTA read the other one back, two threads a row, 32 columns at a time.  Bound by the tensor cores; the tally (some
 // 3000 cycles a tile) hides behind the next tile's products where K is 512 and more.
-// Up to 128 rows: a tile is one CTA's and bound by W's way from HBM.  An SM's share of the bandwidth depends on its die (of two
+// Up to 128 rows: a tile is one CTA's and bound by W's way from HBM, and for long by the power that memory and products draw together:
+// up to 64 rows are multiplied by instructions of 64 (45 x 2048 x 151936, sustained: 103 us, 106 with 128; 1 x 4096: 194 us and 199).  An SM's share of the bandwidth depends on its die (of two
 // equal shares one was read in 176 us, the other in 203), so a CTA that is done takes over one that has not started.
 //
 //   one B200             floor   time        (us; 6536 GB/s, 1670 TFLOP/s)
@@ -45,7 +46,7 @@ __device__ int g_head_error = 0;
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
   int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
-  int zeros;                                          // the others are zeros
+  int m_rows, zeros;                                  // rows of an instruction of a single CTA, 64 or 128; the others are zeros
   const bf16* h;
   int64_t ldh;
   const bf16* w;
@@ -86,8 +87,8 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
   const int units = p.m_tiles * p.n_tiles, k_blocks = (p.K + kHeadK - 1) / kHeadK;
   const int w_rows = PAIR ? p.cols / 2 : p.cols;                                  // of W that this CTA loads for a tile
-  constexpr int a_bytes = kHeadRows * kHeadK * 2;
-  const int block_bytes = a_bytes + w_rows * kHeadK * 2, loaded = block_bytes - (kHeadRows - p.a_box) * kHeadK * 2;       // of a K block
+  const int a_bytes = (PAIR ? kHeadRows : p.m_rows) * kHeadK * 2;
+  const int block_bytes = a_bytes + w_rows * kHeadK * 2, loaded = (p.a_box + w_rows) * kHeadK * 2;       // of a K block
   const int stage_bytes = p.per_stage * block_bytes;
 
   if (threadIdx.x == 0) {
@@ -108,7 +109,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   // memory needs (one row x 4096 x 151936, sustained: 201 us at 1.4 GHz, 214 us at 0.86 GHz without).  Not where a call is too short
   // for that to count, but not for the writing (64 x 512 x 32003: 15.3 us, 14.6 without).
   if (p.zeros) {
-    const int vecs = (kHeadRows - p.a_box) * 8, blocks = p.stages * p.per_stage;
+    const int vecs = a_bytes / 16 - p.a_box * 8, blocks = p.stages * p.per_stage;
     uint4* at = reinterpret_cast<uint4*>(smem + p.a_box * kHeadK * 2) + threadIdx.x;
     for (int b = 0; b < blocks; ++b, at += block_bytes / 16)
       for (int i = threadIdx.x; i < vecs; i += kHeadThreads) at[i - threadIdx.x] = make_uint4(0, 0, 0, 0);
@@ -191,7 +192,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   } else if (warp == 1) {
     if (rank == 0) {
       // ---------------------------------------------------------------- products (a pair's first CTA)
-      const uint32_t id = PAIR ? idesc_pair(p.cols) : idesc(false, p.cols);
+      const uint32_t id = PAIR ? idesc_pair(p.cols) : idesc(false, p.cols, p.m_rows);
       int stage = 0, t = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -232,12 +233,15 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     // ------------------------------------------------------------------ tallies, two threads a row: every other 32 columns
     const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t leader_tempty = PAIR ? in_cta(tempty_bar(0), 0) : 0u;
-    const auto row_of = [&](int m) { return m * 2 * kHeadRows + (int)rank * kHeadRows + q * 32; };
+    // of an instruction of 64 rows, 16 lie in every 32 lanes of tensor memory
+    const bool half_rows = !PAIR && p.m_rows == 64;
+    const auto row_of = [&](int m) { return m * 2 * kHeadRows + (int)rank * kHeadRows + q * (half_rows ? 16 : 32); };
+    const int lane_row = half_rows && lane >= 16 ? p.T : lane;       // or none
     // a row's token and temperature are fetched a tile ahead
     int64_t id_next = -1;
     float c_next = kLog2e;
     const auto fetch = [&](int m) {
-      const int row = row_of(m) + lane;
+      const int row = row_of(m) + lane_row;
       id_next = row < p.T ? p.ids[row] : -1;
       c_next = row < p.T ? row_scale(p.temperature, row) * kLog2e : kLog2e;
     };
@@ -248,7 +252,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
       m = m_next;
       n = PAIR ? n_next : u;
-      const int row0 = row_of(m), row = row0 + lane, n0 = n * p.cols, acc = t & 1;
+      const int row0 = row_of(m), row = row0 + lane_row, n0 = n * p.cols, acc = t & 1;
       const float c = c_next;
       const int64_t want = id_next - n0;              // the given token's column, if it is one of this tile's
       if (PAIR && u + (int)(gridDim.x >> 1) < units) {
@@ -475,12 +479,13 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   // a stage costs the issuing warps some 370 cycles whatever it holds: two K blocks where they are small (64 x 1024 x 32768: 17.5 us,
   // 19.0 with one; 128 rows in tiles of 208 columns, 4096 x 151936: 211 us, 199 with one)
   const int per_stage = a_box + w_box <= 192 ? 2 : 1;
-  int stages = kHeadRing / (per_stage * (kHeadRows + w_box) * kHeadK * 2);
+  const int m_rows = rows <= 64 ? 64 : kHeadRows;
+  int stages = kHeadRing / (per_stage * (m_rows + w_box) * kHeadK * 2);
   if (stages > kHeadMostStages) stages = kHeadMostStages;
   float4* tallies = (float4*)workspace;
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
-  const int zeros = a_box < kHeadRows && (int64_t)vocab * width > (64 << 20);
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, zeros, (const bf16*)hidden, ldh,
+  const int zeros = a_box < m_rows && (int64_t)vocab * width > (64 << 20);
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, m_rows, zeros, (const bf16*)hidden, ldh,
                      (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;

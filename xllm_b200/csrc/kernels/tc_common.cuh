@@ -68,10 +68,10 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
   d |= (uint64_t)2 << 61;
   return d;
 }
-// D = f32, A = B = bf16, M = 128, N = n; b_mn: B is MN-major (bit 16)
-__host__ __device__ constexpr uint32_t idesc(bool b_mn, int n) {
+// D = f32, A = B = bf16, M = 128 or 64, N = n; b_mn: B is MN-major (bit 16)
+__host__ __device__ constexpr uint32_t idesc(bool b_mn, int n, int m = 128) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t id, uint32_t accumulate) {
   asm volatile(
