@@ -116,13 +116,9 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    if constexpr (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    }
+    asm volatile("tcgen05.alloc.cta_group::%1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)), "n"(PAIR ? 2 : 1)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::%0.sync.aligned;" ::"n"(PAIR ? 2 : 1));
   }
   tc_fence_before();
   __syncthreads();
@@ -344,8 +340,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   if constexpr (PAIR) cluster_sync();                 // neither CTA leaves while the other may touch its barriers or memory
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
+    asm volatile("tcgen05.dealloc.cta_group::%1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base), "n"(PAIR ? 2 : 1));
   }
 }
 
