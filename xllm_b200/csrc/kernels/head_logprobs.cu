@@ -14,13 +14,19 @@
 // equal shares one was read in 176 us, the other in 203), so a CTA that is done takes over one that has not started.
 //
 //   one B200             floor   time        (us; 6536 GB/s, 1670 TFLOP/s)
-//   1 x 4096 x 151936      190    193        6.4 TB/s
+//   1 x 4096 x 151936      190    192        6.5 TB/s
 //   45 x 2048 x 151936      95    100
 //   128 x 4096 x 151936    191    199
-//   200 x 4096 x 151936    191    239        of a pair's equal shares; takeover by pairs 252, 256 rows on a single CTA 257
+//   200 x 4096 x 151936    191    240        power, of memory and products of 256 rows; takeover by pairs 250, 256 rows on a single CTA 257
 //   1000 x 4096 x 32768    161    181
 //   4096 x 512 x 151936    382    449        the tally
 //   4096 x 4096 x 151936  3053   3080        0.99 of the burst rate
+//
+// The tensor cores cut a sum of products off at each of its K / 16 steps: measured against 64 bits, scores of dense rows come out
+// smaller by 0.94e-9 K of themselves, at any size, K from 256 to 7168 (0.83 to 1.00e-9; 4.0e-6 at 4096), beside an error half as large.  The
+// tallies take them longer by that, through the factor of their exponents (kHeadCut), and the given tokens' scores are summed once more
+// as fp32 products that round.  Off against 64 bits, relative, 1000 x 4096 x 32768: log-probabilities 1.5e-6, with the rounded sums 9.8e-7,
+// with both 5e-8 (a product in fp32 3.5e-7).  Sums that are not cut, of states with few values other than 0, are longer by that instead.
 //
 // Every wait is bounded; on expiry the kernel raises an error word, all roles leave their loops, tensor memory is freed and the
 // kernel returns.
@@ -40,12 +46,15 @@ constexpr int kHeadFixed = 2 * 16 + kHeadBars * 8 + 16;                // behind
 constexpr int kHeadSmem = kHeadRing + kHeadFixed + kHeadRows * sizeof(Tally) + 1024;
 static_assert(kHeadSmem <= 232448, "exceeds the 227 KB of shared memory per CTA");
 
+constexpr float kHeadCut = 0.94e-9f;
+
 __device__ int g_head_error = 0;
 
 // workspace: tallies (m, z, s, -) [rows][column tiles] and the given tokens' scores [rows], as the tensor cores and as fp32 sums give them
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
   int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
+  float gain;                                         // 1 + kHeadCut K
   int m_rows, zeros;                                  // rows of an instruction of a single CTA, 64 or 128; the others are zeros
   const bf16* h;
   int64_t ldh;
@@ -239,7 +248,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     const auto fetch = [&](int m) {
       const int row = row_of(m) + lane_row;
       id_next = row < p.T ? p.ids[row] : -1;
-      c_next = row < p.T ? row_scale(p.temperature, row) * kLog2e : kLog2e;
+      c_next = (row < p.T ? row_scale(p.temperature, row) : 1.f) * p.gain * kLog2e;
     };
     int t = 0, m, n, m_next, n_next;
     bool ok = true;
@@ -255,8 +264,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
         head_tile(p, u + (gridDim.x >> 1), m_next, n_next);
         if (m_next != m) fetch(m_next);
       }
-      // The tensor cores' sums of K products are cut off at every step, some 2^-19 of a large score in all.  While the tile is
-      // computed, the given tokens' scores are summed once more as fp32 products that round: a warp a row, shared out by the tiles.
+      // While the tile is computed, the given tokens' scores are summed with rounding: a warp a row, shared out by the tiles.
       constexpr int warps = PAIR ? 2 * kHeadWarps : kHeadWarps;
       for (int64_t r = (int64_t)u * warps + (int)rank * kHeadWarps + warp - 2; r < p.T; r += (int64_t)units * warps) {
         const int64_t id = p.ids[r];
@@ -351,10 +359,10 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   const int t = threadIdx.x % threads, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * (256 / threads) + threadIdx.x / threads;
   if (row >= p.T) return;                            // whole warps; no block is left by some of the threads of a row
-  const float scale = row_scale(p.temperature, row), c = scale * kLog2e;
+  const float scale = row_scale(p.temperature, row) * p.gain, c = scale * kLog2e;
   const int64_t id = p.ids[row];
   const bool given = id >= 0 && id < p.V;
-  const float x0 = given ? p.given[row] : 0.f, x = given ? p.summed[row] : 0.f;
+  const float x0 = given ? p.given[row] : 0.f, x = given ? p.summed[row] / p.gain : 0.f;       // in the tallies' scores' size
   const float4* tallies = p.tallies + row * p.n_tiles;
   Tally a = tally_empty();
   for (int i = t; i < p.n_tiles; i += 4 * threads) {
@@ -480,7 +488,7 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   float4* tallies = (float4*)workspace;
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
   const int zeros = a_box < m_rows && (int64_t)vocab * width > (64 << 20);
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, m_rows, zeros, (const bf16*)hidden, ldh,
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, 1.f + kHeadCut * width, m_rows, zeros, (const bf16*)hidden, ldh,
                      (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;
