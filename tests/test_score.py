@@ -252,6 +252,8 @@ def test_refusals():
     for bad in (w[:, :8], w.float(), w.T, w[:0], w[0]):
         with pytest.raises(ValueError):
             score.head_logprobs(h, bad, ids)
+    with pytest.raises(ValueError):
+        score.head_logprobs(h[:, :0], w[:, :0], ids)
     with pytest.raises(TypeError):
         score.head_logprobs(h, w, ids[:2])
 

@@ -132,11 +132,10 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     """The log-probabilities and entropies of token_logprobs(hidden @ weight^T, ids) without the logits: hidden [rows, width]
     and weight [vocab, width] bf16, the products' sums fp32 and never rounded to bf16 (so not the bits of the two steps, which
     round every logit).  Returns (logprob, entropy) fp32 [rows].  A workspace of 16 bytes for each row and up to 256 tokens of
-    the vocabulary is allocated.  On CUDA the width is a multiple of 8 and rows start on
-    16-byte boundaries."""
+    the vocabulary is allocated.  On CUDA the width is a multiple of 8 and rows start on 16-byte boundaries."""
     rows, width, dev = _check_rows(hidden, ids, temperature, "head_logprobs")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.stride(-1) != 1 or weight.dtype != hidden.dtype \
-            or weight.shape[0] < 1 or weight.device != hidden.device:
+            or weight.shape[0] < 1 or width < 1 or weight.device != hidden.device:
         raise ValueError(f"head_logprobs: weight [vocab, {hidden.shape[1]}] {hidden.dtype} on {hidden.device} expected, got "
                          f"{tuple(weight.shape)} {weight.dtype} on {weight.device}")
     vocab = weight.shape[0]
@@ -160,7 +159,7 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     entropy = torch.empty_like(lp)
     work = torch.empty(_head_workspace(rows, vocab, width), dtype=torch.uint8, device=dev)
     check(_lib.load().xllm_head_logprobs(ptr(hidden), _stride(hidden), ptr(weight), _stride(weight), rows, vocab, width, ptr(ids),
-                                 ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream_on(index)), "head_logprobs")
+                                         ptr(temperature), ptr(work), ptr(lp), ptr(entropy), stream_on(index)), "head_logprobs")
     _count(2)
     return lp, entropy
 
