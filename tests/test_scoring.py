@@ -1,6 +1,7 @@
 """Prompts scored end to end: lengths -> tables of the passes -> model -> log-probabilities (`LLM.score`, `/v1/score`)."""
 import json
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -8,7 +9,9 @@ import torch
 from xllm_b200 import LLM
 from xllm_b200.api import scoring
 from xllm_b200.api.embedding import hidden_states
+from xllm_b200.engine.fault import DeviceWatchdog
 from xllm_b200.engine.llm_engine import EngineConfig, LLMEngine
+from xllm_b200.ops import _lib
 
 DEVICES = ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)]
 
@@ -54,6 +57,20 @@ def compare(eng, lists, scores, n_top, tol, temperature=1.0):
 # sum over 256 products of states that differ by bf16 steps (2^-9 relative, some 20 independent ones on the way), and rounds to bf16 once
 # more in the plain form: 2^-9 of scores up to 4, so up to 0.04 in all.
 TOL = {"cpu": 2e-4, "cuda:0": 0.05}
+
+
+def test_watchdog_reads_the_error_word(monkeypatch):
+    """A wait that expired in head_logprobs is a finding like one in a product; a library without it is none."""
+    class Library:
+        xllm_fmha_error_status = xllm_talk_error_status = xllm_gemm_error_status = xllm_gemm_few_error_status = lambda self: 0
+        xllm_head_logprobs_error_status = lambda self: 1
+
+    found, eng = [], SimpleNamespace(device=torch.device("cuda", 0), ps=SimpleNamespace(comm=None))
+    monkeypatch.setattr(_lib, "load", lambda *a: Library())
+    dog = DeviceWatchdog.for_engine(eng, found.append)
+    assert not dog.check() and found == ["head_logprobs: a bounded wait expired (status 1)"]
+    monkeypatch.delattr(Library, "xllm_head_logprobs_error_status")
+    assert DeviceWatchdog.for_engine(eng).check()
 
 
 @pytest.mark.parametrize("device", DEVICES)
