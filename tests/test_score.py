@@ -345,6 +345,21 @@ def test_head_edges(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,K,V", [(40, 512, 3000), (150, 1000, 3000)])
+@pytest.mark.parametrize("low", [1e-5, 1e-7, 1e-9, 1e-30])
+def test_head_lowest_temperatures(device, T, K, V, low):
+    """A token ahead of all others by 0.01 is certain at temperatures that magnify the sums' own rounding to more than the others are
+    behind.  What is left is the rounding of a term of up to 2^1 taken out of its own logarithm: an exponential, a sum, a
+    logarithm, a quotient and a product, 2^-22 each at most."""
+    h, w, _, _ = head_case(T, K, V, 11, device)
+    best = (h.double().cpu() @ w.double().cpu().T).topk(2)
+    sure = best.values[:, 0] - best.values[:, 1] > 0.01
+    assert sure.sum() > T // 2
+    lp, ent = score.head_logprobs(h, w, best.indices[:, 0].to(device), temperature=torch.full((T,), low, device=device))
+    assert lp.cpu()[sure].abs().max() <= 2.0 ** -19 and ent.cpu()[sure].abs().max() <= 2.0 ** -19
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_head_strides(device):
     h, w, ids, t = head_case(9, 128, 333, 4, device)
     want = score.head_logprobs(h, w, ids, temperature=t)

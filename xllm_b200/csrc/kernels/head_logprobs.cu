@@ -390,11 +390,15 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   if (t != 0) return;
   float lp = id < 0 ? 0.f : -INFINITY;
   if (given) {
-    // the given token's term as it was tallied makes way for the one of its rounded sum
-    const float t0 = bounded((x0 - a.m) * c), t1 = bounded((x - a.m) * c), e0 = exp2_fast(t0), e1 = exp2_fast(t1);
-    a.z += e1 - e0;
-    a.s += e1 * t1 - e0 * t0;
-    lp = tally_logprob(a, x, scale);
+    // The given token's term as it was tallied makes way for the one of its rounded sum.  Not where the two lie more than a bit apart: there
+    // the temperature magnifies what the sums are off by, and the term would no longer be one of those that the tally is made of.
+    const bool apart = fabsf((x - x0) * c) > 1.f;
+    if (!apart) {
+      const float t0 = bounded((x0 - a.m) * c), t1 = bounded((x - a.m) * c), e0 = exp2_fast(t0), e1 = exp2_fast(t1);
+      a.z += e1 - e0;
+      a.s += e1 * t1 - e0 * t0;
+    }
+    lp = tally_logprob(a, apart ? x0 : x, scale);
   }
   out_lp[row] = lp;
   out_entropy[row] = tally_entropy(a);
