@@ -360,6 +360,29 @@ def test_head_lowest_temperatures(device, T, K, V, low):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("low", [1e-30, 5e-39, 2e-39, 1e-44])
+def test_temperatures_without_an_inverse(device, low):
+    """The inverse of what fp32 holds below 2.9e-39 is beyond fp32: the most likely token is certain all the same, the others never occur,
+    and of two alike each has half."""
+    x = torch.tensor([[3.0, -1.0, 2.0, -math.inf, 0.5], [1.0, 4.0, 4.0, 0.0, -8.0]]).repeat(2, 1).to(device)
+    ids = torch.tensor([0, 1, 2, 3], device=device)
+    t = torch.full((4,), low, device=device)
+    lp, ent, top, top_lp = score.token_logprobs(x, ids, 2, temperature=t)
+    half = math.log(0.5)
+    near(lp[:2], torch.tensor([0.0, half]), 2.0 ** -20, "logprob")                # a logarithm and its sum
+    assert (lp[2:] < -1e29).all() and top.tolist() == [[0, 2], [1, 2]] * 2
+    near(ent, torch.tensor([0.0, -half] * 2), 2.0 ** -20, "entropy")
+    near(top_lp[:, 0], torch.tensor([0.0, half] * 2), 2.0 ** -20, "alternatives")
+    h = torch.eye(16, dtype=torch.bfloat16, device=device)[:4]
+    w = torch.zeros(5, 16, dtype=torch.bfloat16, device=device)
+    w[:, :4] = torch.where(x == -math.inf, -50.0, x).T.to(torch.bfloat16)
+    lp, ent = score.head_logprobs(h, w, ids, temperature=t)
+    near(lp[:2], torch.tensor([0.0, half]), 2.0 ** -20, "logprob")
+    assert (lp[2:] < -1e29).all()
+    near(ent, torch.tensor([0.0, -half] * 2), 2.0 ** -20, "entropy")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_head_strides(device):
     h, w, ids, t = head_case(9, 128, 333, 4, device)
     want = score.head_logprobs(h, w, ids, temperature=t)

@@ -70,10 +70,11 @@ __device__ __forceinline__ void pair_add(PairTally& a, f32x2 x, float c) {      
 }
 __device__ __forceinline__ Tally pair_sum(const PairTally& a) { return {a.m, a.z.x + a.z.y, a.s.x + a.s.y}; }
 
-// 1 / temperature of a row; c is log2(e) times it
+// 1 / temperature of a row; c is log2(e) times it.  Both are finite: below 2.9e-39 the inverse would not be, and what is 0 behind the
+// maximum would be NaN; a temperature that low leaves the same tokens as 5e-39.
 __device__ __forceinline__ float row_scale(const float* temperature, int64_t row) {
   const float t = temperature ? temperature[row] : 1.f;
-  return t > 0.f ? 1.f / t : 1.f;
+  return t > 0.f ? 1.f / fmaxf(t, 5e-39f) : 1.f;
 }
 // in nats: the type's lowest value as a score leaves fp32's range when scaled to bits
 __device__ __forceinline__ float tally_logprob(const Tally& a, float x, float scale) {
