@@ -283,6 +283,16 @@ def test_refusals_gpu():
         score.head_logprobs(h[:, :16].contiguous(), w[:, :16].contiguous().cpu(), ids)
 
 
+def test_too_many_rows():
+    """More than a kernel counts in 32 bits, of one row in memory."""
+    n = 2 ** 32 + 5
+    x, ids = torch.zeros(1, 8, dtype=torch.bfloat16).expand(n, -1), torch.zeros(1, dtype=torch.int64).expand(n)
+    with pytest.raises(ValueError):
+        score.token_logprobs(x, ids)
+    with pytest.raises(ValueError):
+        score.head_logprobs(x, x[:3], ids)
+
+
 # ------------------------------------------------------------------------------- from hidden states
 def head_case(T, K, V, seed, device, spread=1.4):
     g = torch.Generator().manual_seed(seed)

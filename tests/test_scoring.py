@@ -126,7 +126,8 @@ def test_llm_and_refusals():
     from xllm_b200.api import c_bridge
     got = json.loads(c_bridge.call(llm, "score", json.dumps({"prompts": lists, "top_logprobs": 1})))
     assert got[1]["logprobs"][1:] == outs[1].logprobs[1:] and got[1]["top_logprobs"][1][0] == list(outs[1].top_logprobs[1][0])
-    for bad in (dict(top_logprobs=129), dict(top_logprobs=-1), dict(temperature=0.0), dict(temperature=float("nan"))):
+    for bad in (dict(top_logprobs=129), dict(top_logprobs=-1), dict(temperature=0.0), dict(temperature=float("nan")),
+                dict(temperature=1e-50), dict(temperature=float("inf"))):
         with pytest.raises(ValueError):
             llm.score(lists, **bad)
     for bad in ([[1, 2, 32000]], [[-1]], [[1] * 129]):

@@ -129,7 +129,8 @@ def test_refusals():
     tables.step_tables(**ok)
     for change, error in ((dict(block_table=i32(2, 3).long()), TypeError), (dict(block_table=i32(3, 2).T), TypeError),
                           (dict(ctx_lens=i32(3)), TypeError), (dict(q_lens=i32(2).long()), TypeError), (dict(free_blocks=i32(5).long()), TypeError),
-                          (dict(free_blocks=i32(5, 1)), TypeError), (dict(page=0), ValueError), (dict(page=(1 << 32) + 16), ValueError), (dict(n_rows=-1), ValueError),
+                          (dict(free_blocks=i32(5, 1)), TypeError), (dict(free_blocks=i32(1).expand(1 << 32)), TypeError),
+                          (dict(page=0), ValueError), (dict(page=(1 << 32) + 16), ValueError), (dict(n_rows=-1), ValueError),
                           (dict(block_table=i32(1, 3).expand(2, -1)), ValueError), (dict(block_table=i32(2, 0)), ValueError), (dict(block_table=i32(0, 3), ctx_lens=i32(0), q_lens=i32(0)), ValueError),
                           (dict(block_table=i32(8193, 1), ctx_lens=i32(8193), q_lens=i32(8193)), ValueError)):
         with pytest.raises(error):

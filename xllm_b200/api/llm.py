@@ -391,7 +391,7 @@ class LLM:
 
     def score(self, prompts, top_logprobs: int = 0, temperature: Optional[float] = None) -> List[ScoreOutput]:
         """Log-probability of every token of every prompt under softmax(logits / temperature), with its distribution's entropy and
-        `top_logprobs` alternatives; nothing is generated.  Prompts are strings or token ids; short ones share passes."""
+        `top_logprobs` alternatives; nothing is generated.  A temperature is 1e-6 to 1e6.  Prompts are strings or token ids; short ones share passes."""
         from .scoring import score_token_lists
         if isinstance(prompts, (str, torch.Tensor)) or (prompts and isinstance(prompts[0], int)):
             prompts = [prompts]

@@ -93,8 +93,8 @@ def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperat
         raise ValueError("scoring needs a scratch cache for everything a model keeps per token: this one has an index cache of its own")
     if not 0 <= n_top <= min(score.MAX_TOP, vocab):
         raise ValueError(f"0 to {min(score.MAX_TOP, vocab)} alternatives, asked for {n_top}")
-    if temperature is not None and not temperature > 0:
-        raise ValueError(f"a temperature above 0, not {temperature}")
+    if temperature is not None and not 1e-6 <= temperature <= 1e6:      # results stay finite, as JSON needs them
+        raise ValueError(f"a temperature of 1e-6 to 1e6, not {temperature}")
     for p in prompts:
         if len(p) > engine.max_model_len:
             raise ValueError(f"a prompt of {len(p)} tokens, the model takes {engine.max_model_len}")

@@ -750,7 +750,6 @@ class ApiServer:
                                  "created": int(time.time()), "model": self.model_name, "choices": choices,
                                  "usage": {"prompt_tokens": len(ids), "total_tokens": len(ids)}})
 
-    # ------------------------------------------------------------------ output events
     def _score(self, req, body):
         """Log-probabilities of the prompts' own tokens: `prompt` (text, token ids, or a list of either), `logprobs` alternatives."""
         from .scoring import score_token_lists
@@ -776,6 +775,7 @@ class ApiServer:
         self._json(req.id, 200, {"id": body.get("request_id") or "score-" + str(req.id), "object": "score", "created": int(time.time()),
                                  "model": self.model_name, "choices": choices, "usage": {"prompt_tokens": n, "total_tokens": n}})
 
+    # ------------------------------------------------------------------ output events
     def _sse(self, call, obj):
         self.http.stream_send(call.http_id, "data: " + json.dumps(obj, ensure_ascii=False) + "\n\n")
 

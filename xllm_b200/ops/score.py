@@ -24,6 +24,7 @@ _lib.register_signature("xllm_head_logprobs_workspace", [I, I, I], L)
 _lib.register_signature("xllm_head_logprobs_error_status", [], I)
 
 MAX_TOP = 128          # alternatives a row can list
+MAX_ROWS = 1 << 30     # of a call: tiles of rows are counted in 32 bits
 
 
 def _results(d, x_id, ids, vocab):
@@ -62,6 +63,8 @@ def _check_rows(x, ids, temperature, name):
     if x.dim() != 2 or x.stride(1) != 1 and x.shape[1] > 1:
         raise ValueError(f"{name}: rows [rows, columns] with adjacent columns expected, got {tuple(x.shape)} strides {x.stride()}")
     n, columns = x.shape
+    if n > MAX_ROWS:
+        raise ValueError(f"{name}: at most {MAX_ROWS} rows, got {n}")
     if ids.dtype is not torch.int64 or ids.shape != (n,) or ids.device != dev:
         raise TypeError(f"{name}: ids are int64 [{n}] on {dev}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
     if temperature is not None and (temperature.dtype is not torch.float32 or temperature.shape != (n,) or temperature.device != dev):

@@ -71,8 +71,9 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
     if not (ctx_lens.dtype is q_lens.dtype is torch.int32 and ctx_lens.shape == q_lens.shape == (B,) and ctx_lens.device == q_lens.device == dev):
         raise TypeError(f"step_tables: ctx_lens and q_lens are int32 [{B}] on {dev}, got {ctx_lens.dtype} {tuple(ctx_lens.shape)} on "
                         f"{ctx_lens.device}, {q_lens.dtype} {tuple(q_lens.shape)} on {q_lens.device}")
-    if free_blocks is not None and (free_blocks.dtype is not torch.int32 or free_blocks.dim() != 1 or free_blocks.device != dev):
-        raise TypeError(f"step_tables: free_blocks is int32 [blocks] on {dev}")
+    if free_blocks is not None and (free_blocks.dtype is not torch.int32 or free_blocks.dim() != 1 or free_blocks.device != dev
+                                    or free_blocks.shape[0] >= 1 << 31):
+        raise TypeError(f"step_tables: free_blocks is int32 [blocks] on {dev}, fewer than 2^31")
     if block_table.stride(0) < width and B > 1:
         raise ValueError(f"step_tables: rows of block_table that lie apart, got strides {block_table.stride()} for {width} entries")
     if not 1 <= B <= MAX_REQUESTS or width < 1 or not 1 <= page < 1 << 31 or not 0 <= n_rows < 1 << 31:
