@@ -181,3 +181,54 @@ def test_route(tmp_path):
     finally:
         srv.shutdown()
         t.join(timeout=5)
+
+
+def state_args(model):
+    from xllm_b200.models import ModelArgs
+    if model == "rwkv7":
+        return ModelArgs(model_type="rwkv7", vocab_size=512, hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=4,
+                         head_dim=16, intermediate_size=128, max_position_embeddings=512, tie_word_embeddings=False, extra={})
+    return ModelArgs(model_type="qwen3_next", vocab_size=512, hidden_size=256, num_hidden_layers=4, num_attention_heads=4, num_key_value_heads=2,
+                     head_dim=64, intermediate_size=512, qk_norm=True, rope_theta=1e6, partial_rotary_factor=0.25, max_position_embeddings=512,
+                     tie_word_embeddings=False,
+                     extra=dict(linear_num_value_heads=4, linear_num_key_heads=2, linear_key_head_dim=64, linear_value_head_dim=64,
+                                linear_conv_kernel_dim=4, full_attention_interval=4))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("model", ["qwen3_next", "rwkv7"])
+@pytest.mark.parametrize("outside", ["score", "embed"])
+def test_full_pool_of_states_is_left_alone(device, model, outside):
+    """As many requests in flight as the pool has states: each keeps its own, bit by bit, while prompts are scored or embedded between
+    the steps, and with it its tokens (on the CPU, where a step's sums have one order)."""
+    from xllm_b200.api.embedding import embed_token_lists
+    eng = LLMEngine(EngineConfig(model=model, device=device, dtype="float32" if device == "cpu" else "bfloat16", num_blocks=64, enable_graph=False, max_seqs_per_batch=2,
+                                 max_tokens_per_batch=64, random_weights=True), model_args=state_args(model))
+    assert eng.model.state.n_slots == 3
+    lists = prompts(9, 14, 5, vocab=512)
+
+    def tokens(tag, between):
+        for i, p in enumerate(lists):
+            eng.add_request(f"{tag}{i}", p, max_tokens=12, ignore_eos=True)
+        got = {}
+        while eng.has_unfinished():
+            for e in eng.step():
+                got.setdefault(e.request_id[1:], []).append(e.token)
+            between()
+        return got
+    want = tokens("r", lambda: None)
+    pool, most = eng.model.state, []
+
+    def states():
+        return [t[:, :pool.n_slots].clone() for t in vars(pool).values() if torch.is_tensor(t)]
+
+    def between():
+        most.append(len(pool.owner))
+        before = states()
+        if outside == "score":
+            scoring.score_token_lists(eng, prompts(7, 30, vocab=512, seed=8), 1)
+        else:
+            embed_token_lists(eng, prompts(7, 30, vocab=512, seed=8))
+        assert len(before) > 1 and all(torch.equal(a, b) for a, b in zip(before, states()))
+    got = tokens("s", between)
+    assert max(most) == pool.n_slots and (device != "cpu" or got == want)

@@ -61,8 +61,7 @@ def _forward(engine, prompts, work, table, free, cache):
     meta = AttentionMetadata(n_decode=0, n_prefill=len(work), slots=step.slots, block_table=table, kv_lens=step.kv_lens, cu_q=step.cu_q,
                              max_q_len=max(n for _, _, n in work), max_kv_len=max(at + n for _, at, n in work))
     if getattr(model, "needs_state", False):            # a scratch state slot, reset for this pass
-        st = model.state
-        meta.state_slots = torch.tensor([getattr(st, "scratch_slot", st.n_slots - 1)], device=dev,
+        meta.state_slots = torch.tensor([model.state.scratch_slot], device=dev,
                                         dtype=torch.int32 if getattr(model, "state_on_device", False) else torch.long)
         meta.state_fresh, meta.seq_bounds = [True], [(0, len(tokens))]
     return model.forward(torch.tensor(tokens, dtype=torch.int64, device=dev), step.positions, meta, cache)

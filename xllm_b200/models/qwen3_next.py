@@ -32,12 +32,12 @@ from ..parallel.state import single
 
 
 class LinearStateCache(StateSlots):
-    """Convolution tails and recurrent states of every linear-attention layer, one slot per running sequence."""
+    """Convolution tails and recurrent states of every linear-attention layer, one slot per running sequence and `scratch_slot`."""
 
     def __init__(self, n_layers, slots, conv_dim, kernel, nv, dk, dv, device, dtype):
         super().__init__(slots)
-        self.conv = torch.zeros(n_layers, slots, conv_dim, kernel - 1, dtype=dtype, device=device)
-        self.rec = torch.zeros(n_layers, slots, nv, dk, dv, dtype=torch.float32, device=device)
+        self.conv = torch.zeros(n_layers, slots + 1, conv_dim, kernel - 1, dtype=dtype, device=device)
+        self.rec = torch.zeros(n_layers, slots + 1, nv, dk, dv, dtype=torch.float32, device=device)
 
 
 class GatedDeltaNet(Module):

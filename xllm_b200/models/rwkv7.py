@@ -43,13 +43,13 @@ class _LayerNorm(Module):
 
 
 class Rwkv7State(StateSlots):
-    """Per running sequence: shift vectors of both mixers and the wkv state of every layer."""
+    """Per running sequence: shift vectors of both mixers and the wkv state of every layer; and those of `scratch_slot`."""
 
     def __init__(self, n_layers, slots, hidden, heads, head_size, device, dtype):
         super().__init__(slots)
-        self.att_shift = torch.zeros(n_layers, slots, hidden, dtype=dtype, device=device)
-        self.ffn_shift = torch.zeros(n_layers, slots, hidden, dtype=dtype, device=device)
-        self.wkv = torch.zeros(n_layers, slots, heads, head_size, head_size, dtype=torch.float32, device=device)
+        self.att_shift = torch.zeros(n_layers, slots + 1, hidden, dtype=dtype, device=device)
+        self.ffn_shift = torch.zeros(n_layers, slots + 1, hidden, dtype=dtype, device=device)
+        self.wkv = torch.zeros(n_layers, slots + 1, heads, head_size, head_size, dtype=torch.float32, device=device)
 
 
 class TimeMix(Module):

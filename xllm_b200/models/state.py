@@ -13,12 +13,14 @@ import torch
 
 class StateSlots:
     """Slot numbers owned by the running sequences (keyed by the scheduler's sequence id: parallel samples of one
-    request have their own state)."""
+    request have their own state).  A pool stores one state more, `scratch_slot`, that no sequence owns: for passes outside
+    the scheduler, which run between the steps of the sequences in flight."""
 
     def __init__(self, n_slots: int):
         self.free = list(range(n_slots - 1, -1, -1))
         self.owner = {}
         self.n_slots = n_slots
+        self.scratch_slot = n_slots
 
     def slot_of(self, seq_id) -> int:
         s = self.owner.get(seq_id)
@@ -37,12 +39,11 @@ class StateSlots:
 class RecurrentStatePool(StateSlots):
     """States of any set of layers, by layer: (heads, key size, value size) is one fp32 matrix state per head, the value
     size stored rounded up to four; a dict {name: (shape, dtype)} is a state of several named parts, of which a part with
-    dtype None is such a matrix state.  One more slot than `n_slots` exists: `scratch_slot`, for passes outside the scheduler.
+    dtype None is such a matrix state.
     Slots are not cleared: a layer ignores what a slot holds when a sequence starts at position 0."""
 
     def __init__(self, shapes: Dict[int, Union[Tuple[int, int, int], dict]], n_slots: int, device):
         super().__init__(n_slots)
-        self.scratch_slot = n_slots
 
         def make(part):
             shape, dtype = self._stored(part)
