@@ -123,6 +123,24 @@ def test_largest():
     check([0], [300000], 1, "cuda")
 
 
+@pytest.mark.gpu
+def test_most_requests_first():
+    """Numbers of requests around the shared memory that a launch gets without asking, in a process that has had no larger call."""
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import sys
+sys.path.insert(0, {os.path.dirname(os.path.abspath(__file__))!r})
+from test_step_tables import check
+for B in (4053, 4074, 4075, 4090, 4096, 4097):
+    check([b % 40 for b in range(B)], [b % 3 for b in range(B)], 16, "cuda", pad=1)
+print("served")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "served" in r.stdout, r.stderr[-2000:]
+
+
 def test_refusals():
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
     ok = dict(block_table=i32(2, 3), ctx_lens=i32(2), q_lens=i32(2), page=16, n_rows=4, free_blocks=i32(5))

@@ -34,6 +34,7 @@ struct StepTablesParams {
 
 constexpr int kTablesThreads = 1024;       // at most
 constexpr int kTablesMaxRequests = 8192;
+constexpr int kTablesStatic = kTablesThreads / 32 * sizeof(long long);
 
 // Exclusive prefix of v over the block and its total; `red` is shared memory for 32 values.  All threads call it.
 __device__ __forceinline__ long long block_prefix(long long v, long long* red, long long& total) {
@@ -165,7 +166,7 @@ XLLM_API int xllm_step_tables(void* block_table, int64_t bt_stride, int B, int w
                      (const int32_t*)free_blocks, n_free, (int32_t*)cu_q, (int32_t*)kv_lens, (int64_t*)positions,
                      (int32_t*)slots, (int64_t*)last_rows, (int32_t*)taken};
   const int smem = B * 12;
-  if (smem > 48 * 1024) {
+  if (smem + kTablesStatic > 48 * 1024) {            // what a block gets without asking is for both kinds of shared memory
     const cudaError_t e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTablesMaxRequests * 12);
     if (e != cudaSuccess) return (int)e;
   }
