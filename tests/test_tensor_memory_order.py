@@ -44,3 +44,21 @@ def test_the_order_is_seen():
     good = "{ if (warp == 1) { asm(\"tcgen05.alloc\"); } pdl_wait(); pdl_launch_dependents(); }"
     bad = "{ pdl_wait(); pdl_launch_dependents(); asm(\"tcgen05.alloc\"); }"
     assert not _late(good) and _late(bad)
+
+
+def _unbounded(body):
+    """Waits without an end between the roles' start and the barrier at the kernel's: a warp whose bounded wait expired has left its role,
+    and who waits for it there waits for good."""
+    start = body.index("if (warp == 0)", body.index("pdl_launch_dependents()"))
+    roles = body[start:body.rindex("__syncthreads()")]
+    return re.findall(r"bar\.sync|barrier\.sync|bar\.red|__syncthreads|cluster_sync|barrier\.cluster", roles)
+
+
+def test_roles_that_may_be_left_wait_with_a_bound():
+    body = dict(_bodies((KERNELS / "head_logprobs.cu").read_text()))["head_tally_kernel"]
+    assert _unbounded(body) == []
+
+
+def test_a_wait_without_a_bound_is_seen():
+    body = "{ pdl_launch_dependents(); if (warp == 0) { f(); } else { if (!ok) break; asm(\"bar.sync 1, 64;\"); } __syncthreads(); g(); }"
+    assert _unbounded(body) == ["bar.sync"] and _unbounded(body.replace("bar.sync", "mbarrier")) == []

@@ -41,7 +41,7 @@ using namespace tc;
 constexpr int kHeadRows = 128, kHeadCols = 256, kHeadK = 64;        // rows of a CTA, most columns of a tile, a K block
 constexpr int kHeadWarps = 8, kHeadThreads = 64 + 32 * kHeadWarps, kHeadMostStages = 16;
 constexpr int kHeadRing = 7 * 32 * 1024;                            // bytes of the ring of stages
-constexpr int kHeadBars = 2 * kHeadMostStages + 8;
+constexpr int kHeadBars = 2 * kHeadMostStages + 16;
 constexpr int kHeadFixed = 2 * 16 + kHeadBars * 8 + 16;                // behind it: answers, barriers, two words; then tallies of 128 rows
 constexpr int kHeadSmem = kHeadRing + kHeadFixed + kHeadRows * sizeof(Tally) + 1024;
 static_assert(kHeadSmem <= 232448, "exceeds the 227 KB of shared memory per CTA");
@@ -89,6 +89,8 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   const auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 2 + a); };
   const auto next_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 4 + a); };       // an answer has arrived
   const auto read_bar = [&](int a) { return bar0 + 8u * (2 * kHeadMostStages + 6 + a); };       // all warps have read it
+  const auto give_bar = [&](int q) { return bar0 + 8u * (2 * kHeadMostStages + 8 + q); };       // one thread's tally of a row lies there
+  const auto took_bar = [&](int q) { return bar0 + 8u * (2 * kHeadMostStages + 12 + q); };      // the row's other thread has read it
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + kHeadRing + 32 + kHeadBars * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
@@ -110,6 +112,10 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
       mbar_init(tempty_bar(a), PAIR ? 2 * kHeadWarps : kHeadWarps);
       mbar_init(next_bar(a), 1);
       mbar_init(read_bar(a), 2 + kHeadWarps);
+    }
+    for (int q = 0; q < 4; ++q) {
+      mbar_init(give_bar(q), 1);
+      mbar_init(took_bar(q), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -250,7 +256,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
       id_next = row < p.T ? p.ids[row] : -1;
       c_next = (row < p.T ? row_scale(p.temperature, row) : 1.f) * p.gain * kLog2e;
     };
-    int t = 0, m, n, m_next, n_next;
+    int t = 0, m, n, m_next, n_next, given_over = 0;
     bool ok = true;
     head_tile(p, first, m_next, n_next);
     fetch(m_next);
@@ -329,16 +335,19 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
             if (here) p.given[row] = x;
           }
         }
-        // the row's other thread: a barrier for the two warps, and one more before its place is written again
-        Tally a = pair_sum(run);
+        // One thread of the row gives its tally to the other.  Bounded like every wait: a warp that has left its role is not waited for.
+        const Tally a = pair_sum(run);
         Tally* other = reinterpret_cast<Tally*>(smem + kHeadRing + kHeadFixed) + q * 32 + lane;
-        if (half == 1) *other = a;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
-        if (half == 0) {
-          a = tally_join(a, *other, c);
-          if (row < p.T) p.tallies[(int64_t)row * p.n_tiles + n] = make_float4(a.m, a.z, a.s, 0.f);
+        const uint32_t parity = given_over++ & 1;
+        if (!mbar_wait_warp(half == 1 ? took_bar(q) : give_bar(q), half == 1 ? parity ^ 1 : parity, abort_flag)) break;
+        if (half == 1) {
+          *other = a;
+        } else {
+          const Tally both = tally_join(a, *other, c);
+          if (row < p.T) p.tallies[(int64_t)row * p.n_tiles + n] = make_float4(both.m, both.z, both.s, 0.f);
         }
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(half == 1 ? give_bar(q) : took_bar(q));
       }
     }
   }
