@@ -62,3 +62,11 @@ def test_roles_that_may_be_left_wait_with_a_bound():
 def test_a_wait_without_a_bound_is_seen():
     body = "{ pdl_launch_dependents(); if (warp == 0) { f(); } else { if (!ok) break; asm(\"bar.sync 1, 64;\"); } __syncthreads(); g(); }"
     assert _unbounded(body) == ["bar.sync"] and _unbounded(body.replace("bar.sync", "mbarrier")) == []
+
+
+def test_copies_in_flight_are_waited_for_whoever_gave_up():
+    """A role that gives up leaves others behind that have just started a copy or a product: all of them wait, for a bounded time, behind the
+    barrier at the end and before memory goes."""
+    body = dict(_bodies((KERNELS / "head_logprobs.cu").read_text()))["head_tally_kernel"]
+    end = body[body.rindex("__syncthreads()"):]
+    assert re.search(r"if \(\*abort_flag\) \{\s*const long long t0 = clock64\(\);\s*while \(clock64\(\) - t0 < \d+LL\)", end[:end.index("cluster_sync()")])

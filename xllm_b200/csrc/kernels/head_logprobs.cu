@@ -196,10 +196,6 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
     }
-    if (!ok) {
-      const long long t0 = clock64();
-      while (clock64() - t0 < 20000000LL) {}          // bounded grace period for copies still in flight
-    }
   } else if (warp == 1) {
     if (rank == 0) {
       // ---------------------------------------------------------------- products (a pair's first CTA)
@@ -353,7 +349,11 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_head_error, 1);
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) {}            // copies, products and answers in flight, whichever role gave up
+    if (threadIdx.x == 0) atomicExch(&g_head_error, 1);
+  }
   if constexpr (PAIR) cluster_sync();                 // neither CTA leaves while the other may touch its barriers or memory
   if (warp == 1) {
     tc_fence_after();
