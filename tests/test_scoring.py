@@ -232,3 +232,19 @@ def test_full_pool_of_states_is_left_alone(device, model, outside):
         assert len(before) > 1 and all(torch.equal(a, b) for a, b in zip(before, states()))
     got = tokens("s", between)
     assert max(most) == pool.n_slots and (device != "cpu" or got == want)
+
+
+def test_an_expired_wait_gives_no_scores(monkeypatch):
+    """What head_logprobs returns when a wait of it has expired is not handed out, and the watchdog still hears of it."""
+    class Library:
+        words = [0, 7, 0, 0]
+        xllm_head_logprobs_error_status = lambda self: self.words.pop(0)
+
+    eng = engine("cpu")
+    monkeypatch.setattr(scoring.score, "head_supported", lambda h, w: True)
+    monkeypatch.setattr(scoring.score, "head_logprobs", lambda h, w, ids, temperature=None: (h[:, 0] * math.nan,) * 2)
+    monkeypatch.setattr(_lib, "load", lambda *a: Library())
+    scoring.score_token_lists(eng, prompts(4))
+    with pytest.raises(RuntimeError, match="wait"):
+        scoring.score_token_lists(eng, prompts(4))
+    assert scoring.score.error_status() == 7 and scoring.score.error_status() == 0

@@ -77,12 +77,13 @@ def _score_rows(model, hidden, targets, n_top, temperature):
         h, ids, T = hidden[at:at + step], targets[at:at + step], None if t is None else t[at:at + step]
         parts.append((*score.head_logprobs(h, weight, ids, temperature=T), None, None) if fused else
                      score.token_logprobs(model.logits(h), ids, n_top, temperature=T))
-    return [None if p[0] is None else torch.cat(p) for p in zip(*parts)]
+    return [None if p[0] is None else torch.cat(p) for p in zip(*parts)], fused
 
 
 @torch.no_grad()
 def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperature: Optional[float] = None) -> List[TokenScores]:
-    """Scores of every token of every prompt (token ids), with `n_top` alternatives each, under softmax(logits / temperature)."""
+    """Scores of every token of every prompt (token ids), with `n_top` alternatives each, under softmax(logits / temperature).
+    RuntimeError where a wait of a kernel expired: its scores are not there."""
     model, vocab = engine.model, engine.model.lm_head.vocab
     if engine.asleep:
         raise RuntimeError("the engine is asleep")
@@ -112,8 +113,10 @@ def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperat
             taken = -(-work[0][1] // page)              # blocks of the passes before; 0 where the pass holds several prompts
             hidden = _forward(engine, prompts, work, table, free[taken:], cache)
             given = [t for i, at, n in work for t in (prompts[i] + [-1])[at + 1:at + n + 1]]
-            results = _score_rows(model, hidden, torch.tensor(given, dtype=torch.int64, device=dev), n_top, temperature)
+            results, fused = _score_rows(model, hidden, torch.tensor(given, dtype=torch.int64, device=dev), n_top, temperature)
             lps, ents, top, top_lps = [None if r is None else r.tolist() for r in results]
+            if fused and score.expired():              # behind the copies that waited for it
+                raise RuntimeError("a bounded wait inside head_logprobs expired: no scores")
             row = 0
             for i, at, n in work:
                 m = min(n, len(prompts[i]) - 1 - at)    # the row of a prompt's last token has nothing to score

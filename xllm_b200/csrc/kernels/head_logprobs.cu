@@ -28,8 +28,8 @@
 // as fp32 products that round.  Off against 64 bits, relative, 1000 x 4096 x 32768: log-probabilities 1.5e-6, with the rounded sums 9.8e-7,
 // with both 5e-8 (a product in fp32 3.5e-7).  Sums that are not cut, of states with few values other than 0, are longer by that instead.
 //
-// Every wait is bounded; on expiry the kernel raises an error word, all roles leave their loops, tensor memory is freed and the
-// kernel returns.
+// Every wait is bounded; on expiry the kernel raises an error word and the call's own, all roles leave their loops, tensor memory is
+// freed and the kernel returns.  What the call's tiles would have been is then not there: all its results are NaN.
 #include "logprob_math.cuh"
 #include "tc_common.cuh"
 #include "vec_io.cuh"
@@ -50,7 +50,8 @@ constexpr float kHeadCut = 0.94e-9f;
 
 __device__ int g_head_error = 0;
 
-// workspace: tallies (m, z, s, -) [rows][column tiles] and the given tokens' scores [rows], as the tensor cores and as fp32 sums give them
+// workspace: tallies (m, z, s, -) [rows][column tiles], the given tokens' scores [rows], as the tensor cores and as fp32 sums give them,
+// and whether a wait of this call expired
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
   int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
@@ -65,6 +66,7 @@ struct HeadParams {
   float4* tallies;
   float* given;
   float* summed;
+  int* lost;
 };
 
 // Tile u of the order in which they are worked on: the row tiles of a column tile side by side, so that W is read from HBM once for
@@ -262,6 +264,7 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
       const int row0 = row_of(m), row = row0 + lane_row, n0 = n * p.cols, acc = t & 1;
       const float c = c_next;
       const int64_t want = id_next - n0;              // the given token's column, if it is one of this tile's
+      if (u == 0 && rank == 0 && threadIdx.x == 64) *p.lost = 0;         // long before a wait can expire
       if (PAIR && u + (int)(gridDim.x >> 1) < units) {
         head_tile(p, u + (gridDim.x >> 1), m_next, n_next);
         if (m_next != m) fetch(m_next);
@@ -352,7 +355,10 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
   if (*abort_flag) {
     const long long t0 = clock64();
     while (clock64() - t0 < 20000000LL) {}            // copies, products and answers in flight, whichever role gave up
-    if (threadIdx.x == 0) atomicExch(&g_head_error, 1);
+    if (threadIdx.x == 0) {
+      atomicExch(&g_head_error, 1);
+      atomicExch(p.lost, 1);
+    }
   }
   if constexpr (PAIR) cluster_sync();                 // neither CTA leaves while the other may touch its barriers or memory
   if (warp == 1) {
@@ -409,8 +415,9 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
     }
     lp = tally_logprob(a, apart ? x0 : x, scale);
   }
-  out_lp[row] = lp;
-  out_entropy[row] = tally_entropy(a);
+  const bool lost = *p.lost != 0;
+  out_lp[row] = lost ? NAN : lp;
+  out_entropy[row] = lost ? NAN : tally_entropy(a);
 }
 
 // Columns of a tile: the width whose rounds over the SMs (or pairs of them) and last tally cost least.  A round costs its columns and
@@ -463,7 +470,7 @@ static cudaError_t launch_head_tally(const CUtensorMap& h, const CUtensorMap& w,
 XLLM_API int64_t xllm_head_logprobs_workspace(int rows, int vocab, int width) {
   using namespace xllm;
   const int cols = head_cols(rows, vocab, width);
-  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(float4) + 2 * sizeof(float)) * rows;
+  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(float4) + 2 * sizeof(float)) * rows + sizeof(int);
 }
 
 // Reads and clears the error word: non-zero when a bounded wait expired since the last query.
@@ -502,7 +509,8 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
   const int zeros = a_box < m_rows && (int64_t)vocab * width > (64 << 20);
   const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, 1.f + kHeadCut * width, m_rows, zeros, (const bf16*)hidden, ldh,
-                     (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows};
+                     (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows,
+                     (int*)(given + 2 * (int64_t)rows)};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;
   cudaError_t e = pair ? launch_head_tally<true>(map_h, map_w, p, 2 * (units < 74 ? units : 74), s)

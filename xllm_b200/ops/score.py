@@ -135,7 +135,8 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     """The log-probabilities and entropies of token_logprobs(hidden @ weight^T, ids) without the logits: hidden [rows, width]
     and weight [vocab, width] bf16, the products' sums fp32 and never rounded to bf16 (so not the bits of the two steps, which
     round every logit).  Returns (logprob, entropy) fp32 [rows].  A workspace of 16 bytes for each row and up to 256 tokens of
-    the vocabulary is allocated.  On CUDA the width is a multiple of 8 and rows start on 16-byte boundaries."""
+    the vocabulary is allocated.  On CUDA the width is a multiple of 8 and rows start on 16-byte boundaries.  Where a bounded wait of the
+    kernel expires, all results of the call are NaN and `error_status` tells."""
     rows, width, dev = _check_rows(hidden, ids, temperature, "head_logprobs")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.stride(-1) != 1 or weight.dtype != hidden.dtype \
             or weight.shape[0] < 1 or width < 1 or weight.device != hidden.device:
@@ -167,6 +168,18 @@ def head_logprobs(hidden, weight, ids, temperature=None):
     return lp, entropy
 
 
+_expired = 0           # what `expired` has read and `error_status` has not told yet
+
+
+def expired() -> bool:
+    """Whether a bounded wait inside `head_logprobs` expired; the next `error_status` tells it too."""
+    global _expired
+    _expired |= int(_lib.load().xllm_head_logprobs_error_status())
+    return _expired != 0
+
+
 def error_status() -> int:
     """Non-zero when a bounded wait inside `head_logprobs` expired since the last query."""
-    return int(_lib.load().xllm_head_logprobs_error_status())
+    global _expired
+    v, _expired = _expired | int(_lib.load().xllm_head_logprobs_error_status()), 0
+    return v
