@@ -518,3 +518,14 @@ def test_head_cut_sums(T, K, V):
     for got, want, short in zip(score.head_logprobs(h, w, ids), results(x), results(x * (1 - cut))):
         off, without = (got.double() - want).norm(), (short - want).norm()
         assert float(off) <= 0.25 * float(without) + 8 * STEP * float(want.norm()), (float(off), float(without))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,K,V", [(64, 512, 3000), (100, 64, 700), (300, 1000, 3000)])
+def test_head_signs(device, T, K, V):
+    """A log-probability is not above 0 and an entropy not below, to the last bit: with tokens that are certain, nearly so, and others."""
+    h, w, ids, t = head_case(T, K, V, 17, device)
+    h = (h.float() + torch.linspace(0, 40, T, device=device)[:, None] * w[ids].float()).to(torch.bfloat16)
+    for temperature in (None, t, t * 1e-3):
+        lp, ent = score.head_logprobs(h, w, ids, temperature=temperature)
+        assert bool((lp <= 0).all()) and bool((ent >= 0).all()), (float(lp.max()), float(ent.min()))

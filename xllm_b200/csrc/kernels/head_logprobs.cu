@@ -24,9 +24,8 @@
 //
 // The tensor cores cut a sum of products off at each of its K / 16 steps: measured against 64 bits, scores of dense rows come out
 // smaller by 0.94e-9 K of themselves, at any size, K from 256 to 7168 (0.83 to 1.00e-9; 4.0e-6 at 4096), beside an error half as large.  The
-// tallies take them longer by that, through the factor of their exponents (kHeadCut), and the given tokens' scores are summed once more
-// as fp32 products that round.  Off against 64 bits, relative, 1000 x 4096 x 32768: log-probabilities 1.5e-6, with the rounded sums 9.8e-7,
-// with both 5e-8 (a product in fp32 3.5e-7).  Sums that are not cut, of states with few values other than 0, are longer by that instead.
+// tallies take them longer by that, through the factor of their exponents (kHeadCut).  Sums that are not cut, of states with few values
+// other than 0, are longer by that instead.
 //
 // Every wait is bounded; on expiry the kernel raises an error word and the call's own, all roles leave their loops, tensor memory is
 // freed and the kernel returns.  What the call's tiles would have been is then not there: all its results are NaN.
@@ -50,22 +49,16 @@ constexpr float kHeadCut = 0.94e-9f;
 
 __device__ int g_head_error = 0;
 
-// workspace: tallies (m, z, s, -) [rows][column tiles], the given tokens' scores [rows], as the tensor cores and as fp32 sums give them,
-// and whether a wait of this call expired
+// workspace: tallies (m, z, s, -) [rows][column tiles], the given tokens' scores [rows], and whether a wait of this call expired
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
   int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
   float gain;                                         // 1 + kHeadCut K
   int m_rows, zeros;                                  // rows of an instruction of a single CTA, 64 or 128; the others are zeros
-  const bf16* h;
-  int64_t ldh;
-  const bf16* w;
-  int64_t ldw;
   const int64_t* ids;
   const float* temperature;
   float4* tallies;
   float* given;
-  float* summed;
   int* lost;
 };
 
@@ -269,24 +262,6 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
         head_tile(p, u + (gridDim.x >> 1), m_next, n_next);
         if (m_next != m) fetch(m_next);
       }
-      // While the tile is computed, the given tokens' scores are summed with rounding: a warp a row, shared out by the tiles.
-      constexpr int warps = PAIR ? 2 * kHeadWarps : kHeadWarps;
-      for (int64_t r = (int64_t)u * warps + (int)rank * kHeadWarps + warp - 2; r < p.T; r += (int64_t)units * warps) {
-        const int64_t id = p.ids[r];
-        if (id < 0 || id >= p.V) continue;
-        const bf16 *h = p.h + r * p.ldh, *w = p.w + id * p.ldw;
-        float sum[8] = {};
-#pragma unroll 4
-        for (int k = lane * 8; k < p.K; k += 256) {
-          float a[8], b[8];
-          load_f32<8>(h + k, a);
-          load_f32<8>(w + k, b);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] = fmaf(a[i], b[i], sum[i]);
-        }
-        const float x = warp_sum(((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])));
-        if (lane == 0) p.summed[r] = x;
-      }
       if (!mbar_wait_warp(tfull_bar(acc), (t >> 1) & 1, abort_flag)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + acc * kHeadCols + ((uint32_t)(q * 32) << 16);
@@ -377,7 +352,6 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   const float scale = row_scale(p.temperature, row) * p.gain, c = scale * kLog2e;
   const int64_t id = p.ids[row];
   const bool given = id >= 0 && id < p.V;
-  const float x0 = given ? p.given[row] : 0.f, x = given ? p.summed[row] / p.gain : 0.f;       // in the tallies' scores' size
   const float4* tallies = p.tallies + row * p.n_tiles;
   Tally a = tally_empty();
   for (int i = t; i < p.n_tiles; i += 4 * threads) {
@@ -403,18 +377,8 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
     for (int w = 1; w < 8; ++w) a = tally_join(a, part[w], c);
   }
   if (t != 0) return;
-  float lp = id < 0 ? 0.f : -INFINITY;
-  if (given) {
-    // The given token's term as it was tallied makes way for the one of its rounded sum.  Not where the two lie more than a bit apart: there
-    // the temperature magnifies what the sums are off by, and the term would no longer be one of those that the tally is made of.
-    const bool apart = fabsf((x - x0) * c) > 1.f;
-    if (!apart) {
-      const float t0 = bounded((x0 - a.m) * c), t1 = bounded((x - a.m) * c), e0 = exp2_fast(t0), e1 = exp2_fast(t1);
-      a.z += e1 - e0;
-      a.s += e1 * t1 - e0 * t0;
-    }
-    lp = tally_logprob(a, apart ? x0 : x, scale);
-  }
+  // a given token's score is one of those that the tally is made of: no more than its maximum, so that no log-probability is above 0
+  const float lp = given ? tally_logprob(a, p.given[row], scale) : id < 0 ? 0.f : -INFINITY;
   const bool lost = *p.lost != 0;
   out_lp[row] = lost ? NAN : lp;
   out_entropy[row] = lost ? NAN : tally_entropy(a);
@@ -470,7 +434,7 @@ static cudaError_t launch_head_tally(const CUtensorMap& h, const CUtensorMap& w,
 XLLM_API int64_t xllm_head_logprobs_workspace(int rows, int vocab, int width) {
   using namespace xllm;
   const int cols = head_cols(rows, vocab, width);
-  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(float4) + 2 * sizeof(float)) * rows + sizeof(int);
+  return ((int64_t)((vocab + cols - 1) / cols) * sizeof(float4) + sizeof(float)) * rows + sizeof(int);
 }
 
 // Reads and clears the error word: non-zero when a bounded wait expired since the last query.
@@ -508,9 +472,8 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   float4* tallies = (float4*)workspace;
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
   const int zeros = a_box < m_rows && (int64_t)vocab * width > (64 << 20);
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, 1.f + kHeadCut * width, m_rows, zeros, (const bf16*)hidden, ldh,
-                     (const bf16*)weight, ldw, (const int64_t*)ids, (const float*)temperature, tallies, given, given + rows,
-                     (int*)(given + 2 * (int64_t)rows)};
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, 1.f + kHeadCut * width, m_rows, zeros,
+                     (const int64_t*)ids, (const float*)temperature, tallies, given, (int*)(given + rows)};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;
   cudaError_t e = pair ? launch_head_tally<true>(map_h, map_w, p, 2 * (units < 74 ? units : 74), s)
