@@ -529,3 +529,46 @@ def test_head_signs(device, T, K, V):
     for temperature in (None, t, t * 1e-3):
         lp, ent = score.head_logprobs(h, w, ids, temperature=temperature)
         assert bool((lp <= 0).all()) and bool((ent >= 0).all()), (float(lp.max()), float(ent.min()))
+
+
+def sums_case(kind, T, K, V, device):
+    """Hidden states whose scores' partial sums do not grow evenly over K."""
+    g = torch.Generator().manual_seed(K + T)
+    w = (torch.randn(V, K, generator=g)).to(torch.bfloat16)
+    h = torch.zeros(T, K)
+    if kind == "one":                                                 # one channel other than 0
+        h[torch.arange(T), torch.randint(0, K, (T,), generator=g)] = 6.0
+    elif kind == "few":
+        for r in range(T):
+            h[r, torch.randperm(K, generator=g)[:4]] = 3.0
+    elif kind in ("first", "last"):                                   # one channel far larger than all others
+        h = torch.randn(T, K, generator=g) * 0.1 / math.sqrt(K)
+        h[:, 0 if kind == "first" else K - 1] = 6.0
+    elif kind == "cancel":                                            # the second half takes back most of the first one
+        h = torch.randn(T, K, generator=g) * 12 / math.sqrt(K)
+        h[:, K // 2:] = -h[:, :K // 2]
+        w[:, K // 2:] = (w[:, :K // 2].float() + 0.3 * torch.randn(V, K // 2, generator=g)).to(torch.bfloat16)
+    ids = torch.randint(0, V, (T,), generator=g)
+    return h.to(torch.bfloat16).to(device), w.to(device), ids.to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["one", "few", "first", "last", "cancel"])
+@pytest.mark.parametrize("T,K,V", [(40, 4096, 2000), (150, 4096, 1000), (40, 1536, 2000)])
+def test_head_uneven_sums(device, kind, T, K, V):
+    """Whatever order a score's products come in: no more than 1024 of them are summed in the tensor cores, in 64 steps, each of which cuts
+    off less than 2^-23 of the largest partial sum and half of that on average, so together 64 of 2^-24 of it; and next to nothing
+    of a sum of few products.  A log-probability moves by at most as much as the scores, and has 8 roundings to fp32 of its own."""
+    h, w, ids = sums_case(kind, T, K, V, device)
+    x, partial = torch.zeros(T, V, dtype=torch.float64), torch.zeros(T, dtype=torch.float64)
+    hd, wd = h.double().cpu(), w.double().cpu()
+    for k in range(0, K, 64):
+        x += hd[:, k:k + 64] @ wd[:, k:k + 64].T
+        partial = torch.maximum(partial, x.abs().amax(1))
+    lp = torch.log_softmax(x, dim=1)
+    want = lp.gather(1, ids.cpu()[:, None])[:, 0], -(lp.exp() * lp).sum(1)
+    got = score.head_logprobs(h, w, ids)
+    cut = 0.0 if kind in ("one", "few") else 64 * STEP * float(partial.norm())
+    for a, b, name in zip(got, want, ("logprob", "entropy")):
+        off = float((a.double().cpu() - b).norm())
+        assert off <= cut + 8 * STEP * float(torch.stack(want).abs().amax(0).norm()), (name, off, cut, float(b.norm()))

@@ -22,10 +22,12 @@
 //   4096 x 512 x 151936    382    449        the tally
 //   4096 x 4096 x 151936  3053   3080        0.99 of the burst rate
 //
-// The tensor cores cut a sum of products off at each of its K / 16 steps: measured against 64 bits, scores of dense rows come out
-// smaller by 0.94e-9 K of themselves, at any size, K from 256 to 7168 (0.83 to 1.00e-9; 4.0e-6 at 4096), beside an error half as large.  The
-// tallies take them longer by that, through the factor of their exponents (kHeadCut).  Sums that are not cut, of states with few values
-// other than 0, are longer by that instead.
+// The tensor cores cut a sum of products off at each of its K / 16 steps, by 2^-26 of what is there on average (measured against 64 bits:
+// scores of dense rows come out smaller by 0.94e-9 K of themselves, those of one large channel in front of all others by twice that).  So
+// no more than 1024 products are summed there: longer rows in chunks of up to 896, whose sums are added up in fp32, with rounding, by the
+// threads that read the accumulators.  Off against 64 bits, relative, 1000 x 4096 x 32768: log-probabilities 3.2e-7, entropies 2.0e-7 (a
+// product in fp32 3.5e-7 and 1.4e-7; unchunked 1.5e-6).  For seconds, unchunked and in chunks: 4096 x 4096 x 151936 3636 and 3663 us, in
+// chunks of 512 3823; 4096 x 1536 x 151936 1386 and 1417; 45 x 2048 x 151936 105 and 106.
 //
 // Every wait is bounded; on expiry the kernel raises an error word and the call's own, all roles leave their loops, tensor memory is
 // freed and the kernel returns.  What the call's tiles would have been is then not there: all its results are NaN.
@@ -45,15 +47,14 @@ constexpr int kHeadFixed = 2 * 16 + kHeadBars * 8 + 16;                // behind
 constexpr int kHeadSmem = kHeadRing + kHeadFixed + kHeadRows * sizeof(Tally) + 1024;
 static_assert(kHeadSmem <= 232448, "exceeds the 227 KB of shared memory per CTA");
 
-constexpr float kHeadCut = 0.94e-9f;
+constexpr int kHeadOne = 16, kHeadChunk = 14;                       // most K blocks that are summed in tensor memory: alone, and as a chunk
 
 __device__ int g_head_error = 0;
 
 // workspace: tallies (m, z, s, -) [rows][column tiles], the given tokens' scores [rows], and whether a wait of this call expired
 struct HeadParams {
   int T, V, K, cols, n_tiles, m_tiles;
-  int a_box, per_stage, stages;                       // rows of h that are loaded, K blocks of a stage, stages
-  float gain;                                         // 1 + kHeadCut K
+  int a_box, per_stage, stages, chunk;                // rows of h that are loaded, K blocks of a stage, stages, K blocks of a chunk
   int m_rows, zeros;                                  // rows of an instruction of a single CTA, 64 or 128; the others are zeros
   const int64_t* ids;
   const float* temperature;
@@ -72,7 +73,39 @@ __device__ __forceinline__ void head_tile(const HeadParams& p, int u, int& m, in
   m = g * kHeadGroup + r - n * wide;
 }
 
-template <bool PAIR>
+// adds the first `left` of 32 columns
+__device__ __forceinline__ void tally_columns(PairTally& run, float* x, int left, float c) {
+  if (left < 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i >= left) x[i] = -INFINITY;
+  }
+  float most[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    most[k] = x[k];
+#pragma unroll
+    for (int i = k + 4; i < 32; i += 4) most[k] = fmaxf(most[k], x[i]);
+  }
+  most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+  if (most[0] > run.m) pair_rebase(run, most[0], c);
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) pair_add(run, {x[i], x[i + 1]}, c);
+}
+// x += 32 columns of an accumulator, 16 at a time: the threads that do have no registers to spare, and next to no L1 for what is spilled
+__device__ __forceinline__ void add_columns(uint32_t taddr, float* x) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 16) {
+    uint32_t r[16];
+    tmem_ld16(taddr + k, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[k + i] += __uint_as_float(r[i]);
+  }
+}
+
+// ONE: a row's K blocks are one chunk.
+template <bool PAIR, bool ONE>
 __global__ void __launch_bounds__(kHeadThreads, 1)
 head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -195,40 +228,45 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     if (rank == 0) {
       // ---------------------------------------------------------------- products (a pair's first CTA)
       const uint32_t id = PAIR ? idesc_pair(p.cols) : idesc(false, p.cols, p.m_rows);
-      int stage = 0, t = 0;
+      int stage = 0, t = 0, chunks = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
-        const int acc = t & 1;
-        if (!(PAIR ? mbar_wait_cluster_warp(tempty_bar(acc), ((t >> 1) & 1) ^ 1, abort_flag)
-                   : mbar_wait_warp(tempty_bar(acc), ((t >> 1) & 1) ^ 1, abort_flag))) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d = tmem_base + acc * kHeadCols;
-        for (int kb = 0; kb < k_blocks; kb += p.per_stage) {
-          if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+        for (int kc = 0; kc < k_blocks && ok; kc += p.chunk, ++chunks) {
+          const int acc = chunks & 1, end = min(kc + p.chunk, k_blocks);
+          const uint32_t parity = ((chunks >> 1) & 1) ^ 1;
+          if (!(PAIR ? mbar_wait_cluster_warp(tempty_bar(acc), parity, abort_flag) : mbar_wait_warp(tempty_bar(acc), parity, abort_flag))) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
-          const int blocks = min(p.per_stage, k_blocks - kb);
-          if (elect_one()) {
-            for (int i = 0; i < blocks; ++i) {
-              const uint32_t at = sbase + stage * stage_bytes + i * block_bytes;
-              const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + a_bytes, 16, 1024);
+          const uint32_t d = tmem_base + acc * kHeadCols;
+          for (int kb = kc; kb < end; kb += p.per_stage) {
+            if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const int blocks = min(p.per_stage, end - kb);
+            if (elect_one()) {
+              for (int i = 0; i < blocks; ++i) {
+                const uint32_t at = sbase + stage * stage_bytes + i * block_bytes;
+                const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + a_bytes, 16, 1024);
 #pragma unroll
-              for (int k = 0; k < kHeadK / 16; ++k) {
-                if constexpr (PAIR) umma_pair(d, a + 2 * k, b + 2 * k, id, (kb + i | k) != 0);
-                else umma(d, a + 2 * k, b + 2 * k, id, (kb + i | k) != 0);
+                for (int k = 0; k < kHeadK / 16; ++k) {
+                  if constexpr (PAIR) umma_pair(d, a + 2 * k, b + 2 * k, id, (kb + i - kc | k) != 0);
+                  else umma(d, a + 2 * k, b + 2 * k, id, (kb + i - kc | k) != 0);
+                }
               }
+              if constexpr (PAIR) umma_commit_pair(empty_bar(stage));
+              else umma_commit(empty_bar(stage));
             }
-            if constexpr (PAIR) umma_commit_pair(empty_bar(stage));
-            else umma_commit(empty_bar(stage));
+            __syncwarp();
+            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+          }
+          if (ok && elect_one()) {
+            if constexpr (PAIR) umma_commit_pair(tfull_bar(acc));
+            else umma_commit(tfull_bar(acc));
           }
           __syncwarp();
-          if (++stage == p.stages) { stage = 0; phase ^= 1; }
         }
-        if (ok && elect_one()) {
-          if constexpr (PAIR) umma_commit_pair(tfull_bar(acc));
-          else umma_commit(tfull_bar(acc));
-        }
-        __syncwarp();
       }
     }
   } else {
@@ -245,16 +283,16 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
     const auto fetch = [&](int m) {
       const int row = row_of(m) + lane_row;
       id_next = row < p.T ? p.ids[row] : -1;
-      c_next = (row < p.T ? row_scale(p.temperature, row) : 1.f) * p.gain * kLog2e;
+      c_next = (row < p.T ? row_scale(p.temperature, row) : 1.f) * kLog2e;
     };
-    int t = 0, m, n, m_next, n_next, given_over = 0;
+    int t = 0, chunks = 0, m, n, m_next, n_next, given_over = 0;
     bool ok = true;
     head_tile(p, first, m_next, n_next);
     fetch(m_next);
     for (int u = first; u >= 0 && ok; u = next_unit(u, t, ok), ++t) {
       m = m_next;
       n = PAIR ? n_next : u;
-      const int row0 = row_of(m), row = row0 + lane_row, n0 = n * p.cols, acc = t & 1;
+      const int row0 = row_of(m), row = row0 + lane_row, n0 = n * p.cols;
       const float c = c_next;
       const int64_t want = id_next - n0;              // the given token's column, if it is one of this tile's
       if (u == 0 && rank == 0 && threadIdx.x == 64) *p.lost = 0;         // long before a wait can expire
@@ -262,53 +300,81 @@ head_tally_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_consta
         head_tile(p, u + (gridDim.x >> 1), m_next, n_next);
         if (m_next != m) fetch(m_next);
       }
-      if (!mbar_wait_warp(tfull_bar(acc), (t >> 1) & 1, abort_flag)) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + acc * kHeadCols + ((uint32_t)(q * 32) << 16);
       const int width = min(p.V - n0, p.cols);
-      // the accumulator is free once its last columns are in registers
+      const bool idle = row0 >= p.T || half * 32 >= width;
+      const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16) + half * 32;
+      const auto wait = [&] {
+        if (!mbar_wait_warp(tfull_bar(chunks & 1), (chunks >> 1) & 1, abort_flag)) ok = false;
+        tc_fence_after();
+        return ok;
+      };
+      // the accumulator is free once its columns are in registers
       const auto release = [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_remote(leader_tempty + 8u * acc);
-          else mbar_arrive(tempty_bar(acc));
+          if constexpr (PAIR) mbar_arrive_remote(leader_tempty + 8u * (chunks & 1));
+          else mbar_arrive(tempty_bar(chunks & 1));
         }
       };
-      if (row0 >= p.T || half * 32 >= width) release();
-      if (row0 < p.T) {
-        PairTally run = pair_empty();
-        for (int c0 = half * 32; c0 < width; c0 += 64) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c0, r);
-          tmem_ld_wait();
-          if (c0 + 64 >= width) release();
-          const int left = min(32, width - c0);
-          if (left < 32) {
+      // where the given token is one of 32 columns
+      const auto keep_given = [&](const float* x, int c0, int left) {
+        const bool here = want >= c0 && want < c0 + left;
+        if (!__any_sync(0xffffffffu, here)) return;
+        float v = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= left) r[j] = 0xFF800000u;
-          }
-          float most[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            most[i] = __uint_as_float(r[i]);
-#pragma unroll
-            for (int j = i + 4; j < 32; j += 4) most[i] = fmaxf(most[i], __uint_as_float(r[j]));
-          }
-          most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-          if (most[0] > run.m) pair_rebase(run, most[0], c);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) pair_add(run, {__uint_as_float(r[j]), __uint_as_float(r[j + 1])}, c);
-          const bool here = want >= c0 && want < c0 + left;
-          if (__any_sync(0xffffffffu, here)) {
-            float x = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (want == c0 + j) x = __uint_as_float(r[j]);
-            if (here) p.given[row] = x;
+        for (int i = 0; i < 32; ++i)
+          if (want == c0 + i) v = x[i];
+        if (here) p.given[row] = v;
+      };
+      PairTally run = pair_empty();
+      if constexpr (ONE) {
+        if (!wait()) break;
+        if (idle) {
+          release();
+        } else {
+          const uint32_t taddr = lanes - half * 32 + (chunks & 1) * kHeadCols;
+          for (int c0 = half * 32; c0 < width; c0 += 64) {
+            float x[32];
+            tmem_ld32(taddr + c0, reinterpret_cast<uint32_t*>(x));
+            tmem_ld_wait();
+            if (c0 + 64 >= width) release();
+            const int left = min(32, width - c0);
+            tally_columns(run, x, left, c);
+            keep_given(x, c0, left);
           }
         }
+        ++chunks;
+      } else {
+        // all of the thread's columns, summed over the chunks
+        float x[kHeadCols / 64][32];
+        for (int kc = 0; kc < k_blocks; kc += p.chunk, ++chunks) {
+          if (!wait()) break;
+          const uint32_t taddr = lanes + (chunks & 1) * kHeadCols;
+          if (!idle && kc == 0) {
+#pragma unroll
+            for (int j = 0; j < kHeadCols / 64; ++j)
+              if (half * 32 + 64 * j < width) tmem_ld32(taddr + 64 * j, reinterpret_cast<uint32_t*>(x[j]));
+            tmem_ld_wait();
+          } else if (!idle) {
+#pragma unroll
+            for (int j = 0; j < kHeadCols / 64; ++j)
+              if (half * 32 + 64 * j < width) add_columns(taddr + 64 * j, x[j]);
+          }
+          release();
+        }
+        if (!ok) break;
+        if (!idle) {
+#pragma unroll
+          for (int j = 0; j < kHeadCols / 64; ++j) {
+            const int c0 = half * 32 + 64 * j, left = min(32, width - c0);
+            if (left <= 0) continue;
+            tally_columns(run, x[j], left, c);
+            keep_given(x[j], c0, left);
+          }
+        }
+      }
+      if (row0 < p.T) {
         // One thread of the row gives its tally to the other.  Bounded like every wait: a warp that has left its role is not waited for.
         const Tally a = pair_sum(run);
         Tally* other = reinterpret_cast<Tally*>(smem + kHeadRing + kHeadFixed) + q * 32 + lane;
@@ -349,7 +415,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   const int t = threadIdx.x % threads, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * (256 / threads) + threadIdx.x / threads;
   if (row >= p.T) return;                            // whole warps; no block is left by some of the threads of a row
-  const float scale = row_scale(p.temperature, row) * p.gain, c = scale * kLog2e;
+  const float scale = row_scale(p.temperature, row), c = scale * kLog2e;
   const int64_t id = p.ids[row];
   const bool given = id >= 0 && id < p.V;
   const float4* tallies = p.tallies + row * p.n_tiles;
@@ -402,13 +468,13 @@ static int head_cols(int rows, int vocab, int width) {
   return cols;
 }
 
-template <bool PAIR>
+template <bool PAIR, bool ONE>
 static cudaError_t launch_head_tally(const CUtensorMap& h, const CUtensorMap& w, const HeadParams& p, int ctas, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   static bool attr_done[64] = {};
   if (!attr_done[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(head_tally_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem);
+    const cudaError_t e = cudaFuncSetAttribute(head_tally_kernel<PAIR, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem);
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = true;
   }
@@ -425,7 +491,7 @@ static cudaError_t launch_head_tally(const CUtensorMap& h, const CUtensorMap& w,
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, head_tally_kernel<PAIR>, h, w, p);
+  return cudaLaunchKernelEx(&cfg, head_tally_kernel<PAIR, ONE>, h, w, p);
 }
 
 }  // namespace xllm
@@ -469,15 +535,19 @@ XLLM_API int xllm_head_logprobs(const void* hidden, int64_t ldh, const void* wei
   const int m_rows = rows <= 64 ? 64 : kHeadRows;
   int stages = kHeadRing / (per_stage * (m_rows + w_box) * kHeadK * 2);
   if (stages > kHeadMostStages) stages = kHeadMostStages;
+  // chunks of one length, whole stages each
+  const int k_blocks = (width + kHeadK - 1) / kHeadK, n_chunks = k_blocks <= kHeadOne ? 1 : (k_blocks + kHeadChunk - 1) / kHeadChunk;
+  const int chunk = ((k_blocks + n_chunks - 1) / n_chunks + 1) & ~1;
   float4* tallies = (float4*)workspace;
   float* given = (float*)(tallies + (int64_t)n_tiles * rows);
   const int zeros = a_box < m_rows && (int64_t)vocab * width > (64 << 20);
-  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, 1.f + kHeadCut * width, m_rows, zeros,
+  const HeadParams p{rows, vocab, width, cols, n_tiles, m_tiles, a_box, per_stage, stages, chunk, m_rows, zeros,
                      (const int64_t*)ids, (const float*)temperature, tallies, given, (int*)(given + rows)};
   cudaStream_t s = (cudaStream_t)stream;
   const int units = m_tiles * n_tiles;
-  cudaError_t e = pair ? launch_head_tally<true>(map_h, map_w, p, 2 * (units < 74 ? units : 74), s)
-                       : launch_head_tally<false>(map_h, map_w, p, units, s);
+  const auto launch = n_chunks == 1 ? pair ? launch_head_tally<true, true> : launch_head_tally<false, true>
+                                    : pair ? launch_head_tally<true, false> : launch_head_tally<false, false>;
+  cudaError_t e = launch(map_h, map_w, p, pair ? 2 * (units < 74 ? units : 74) : units, s);
   if (e != cudaSuccess) return (int)e;
   const int threads = rows <= 296 && n_tiles > 128 ? 256 : 32;       // a block a row while that fills the SMs
   e = launch_pdl(head_join_kernel, dim3((unsigned)(((int64_t)rows * threads + 255) / 256)), dim3(256), 0, s, p, threads, (float*)out_lp,
