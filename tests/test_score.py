@@ -293,6 +293,19 @@ def test_too_many_rows():
         score.head_logprobs(x, x[:3], ids)
 
 
+@pytest.mark.parametrize("columns", [(1 << 30) + 1, (1 << 31) - 1, (1 << 32) + 5])
+def test_too_many_columns(columns):
+    """More than a kernel counts in 32 bits; nothing of them is read."""
+    e = lambda *shape, dtype=torch.bfloat16: torch.empty(*shape, dtype=dtype, device="meta")
+    ids = e(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="columns"):
+        score.token_logprobs(e(1, columns), ids)
+    with pytest.raises(ValueError, match="columns"):
+        score.head_logprobs(e(1, columns), e(3, columns), ids)
+    with pytest.raises(ValueError, match="vocabulary"):
+        score.head_logprobs(e(1, 8), e(columns, 8), ids)
+
+
 # ------------------------------------------------------------------------------- from hidden states
 def head_case(T, K, V, seed, device, spread=1.4):
     g = torch.Generator().manual_seed(seed)

@@ -141,6 +141,14 @@ print("served")
     assert r.returncode == 0 and "served" in r.stdout, r.stderr[-2000:]
 
 
+@pytest.mark.parametrize("width", [1 << 31, (1 << 32) + 5])
+def test_too_wide(width):
+    """More entries than a kernel counts in 32 bits; nothing of them is read."""
+    e = lambda *shape: torch.empty(*shape, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="width"):
+        tables.step_tables(e(1, width), e(1), e(1), 16, 4, e(3))
+
+
 def test_refusals():
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
     ok = dict(block_table=i32(2, 3), ctx_lens=i32(2), q_lens=i32(2), page=16, n_rows=4, free_blocks=i32(5))

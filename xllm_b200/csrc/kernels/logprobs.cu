@@ -442,7 +442,7 @@ static int launch_token_logprobs(const ScoreParams& p, int rows, int split, cuda
 // 4096 scores at least (64 x 151936, 20 alternatives: 25.7 us whole, 13.6 in 4 parts, 17.4 in 8; 150 x 32768: 8.0 us whole, 10.1 in 4).
 static int score_split(int rows, int V) {
   int split = 1;
-  while (split < kScoreMaxSplit && rows * split * 2 <= 400 && V / (split * 2) >= 4096) split *= 2;
+  while (split < kScoreMaxSplit && (int64_t)rows * split * 2 <= 400 && V / (split * 2) >= 4096) split *= 2;
   return split;
 }
 

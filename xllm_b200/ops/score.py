@@ -25,6 +25,7 @@ _lib.register_signature("xllm_head_logprobs_error_status", [], I)
 
 MAX_TOP = 128          # alternatives a row can list
 MAX_ROWS = 1 << 30     # of a call: tiles of rows are counted in 32 bits
+MAX_COLUMNS = 1 << 30  # of a row, and tokens of a vocabulary: as are the places in a row
 
 
 def _results(d, x_id, ids, vocab):
@@ -65,6 +66,8 @@ def _check_rows(x, ids, temperature, name):
     n, columns = x.shape
     if n > MAX_ROWS:
         raise ValueError(f"{name}: at most {MAX_ROWS} rows, got {n}")
+    if columns > MAX_COLUMNS:
+        raise ValueError(f"{name}: at most {MAX_COLUMNS} columns, got {columns}")
     if ids.dtype is not torch.int64 or ids.shape != (n,) or ids.device != dev:
         raise TypeError(f"{name}: ids are int64 [{n}] on {dev}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
     if temperature is not None and (temperature.dtype is not torch.float32 or temperature.shape != (n,) or temperature.device != dev):
@@ -143,6 +146,8 @@ def head_logprobs(hidden, weight, ids, temperature=None):
         raise ValueError(f"head_logprobs: weight [vocab, {hidden.shape[1]}] {hidden.dtype} on {hidden.device} expected, got "
                          f"{tuple(weight.shape)} {weight.dtype} on {weight.device}")
     vocab = weight.shape[0]
+    if vocab > MAX_COLUMNS:
+        raise ValueError(f"head_logprobs: a vocabulary of at most {MAX_COLUMNS} tokens, got {vocab}")
     if _debug.enabled():
         _debug.check_range(ids, 0, vocab, "head_logprobs ids", allow_negative_skip=True)
     if not hidden.is_cuda:

@@ -76,8 +76,8 @@ def step_tables(block_table, ctx_lens, q_lens, page, n_rows, free_blocks=None):
         raise TypeError(f"step_tables: free_blocks is int32 [blocks] on {dev}, fewer than 2^31")
     if block_table.stride(0) < width and B > 1:
         raise ValueError(f"step_tables: rows of block_table that lie apart, got strides {block_table.stride()} for {width} entries")
-    if not 1 <= B <= MAX_REQUESTS or width < 1 or not 1 <= page < 1 << 31 or not 0 <= n_rows < 1 << 31:
-        raise ValueError(f"step_tables: 1 to {MAX_REQUESTS} requests, a width and a page of 1 or more and 0 or more rows, got "
+    if not 1 <= B <= MAX_REQUESTS or not 1 <= width < 1 << 31 or not 1 <= page < 1 << 31 or not 0 <= n_rows < 1 << 31:
+        raise ValueError(f"step_tables: 1 to {MAX_REQUESTS} requests, a width and a page of 1 or more and 0 or more rows, all below 2^31, got "
                          f"{B}, {width}, {page}, {n_rows}")
     if _debug.enabled():
         _debug.check_range(ctx_lens, 0, 1 << 31, "step_tables ctx_lens")
