@@ -248,3 +248,22 @@ def test_an_expired_wait_gives_no_scores(monkeypatch):
     with pytest.raises(RuntimeError, match="wait"):
         scoring.score_token_lists(eng, prompts(4))
     assert scoring.score.error_status() == 7 and scoring.score.error_status() == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_alternatives_change_no_score(device):
+    """A token's log-probability and its entropy have the same bits whether alternatives are asked for or not; the alternatives are those of
+    the logits as they are sampled from, on the GPU rounded to bf16: 2^-8 of a logit, and as much of the sum's logarithm."""
+    eng = engine(device)
+    hidden = hidden_states(eng, prompts(300)[0])
+    ids = torch.tensor(prompts(300, seed=5)[0], device=hidden.device)
+    logits = eng.model.logits(hidden)
+    for temperature in (None, 0.6):
+        want, _ = scoring._score_rows(eng.model, hidden, ids, 0, temperature)
+        got, _ = scoring._score_rows(eng.model, hidden, ids, 5, temperature)
+        assert want[2] is None and want[3] is None
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        exact = torch.log_softmax((hidden.double() @ eng.model.lm_head.weight[:logits.shape[1]].double().T) / (temperature or 1.0), dim=1)
+        off = float(logits.abs().max()) / (temperature or 1.0) * (2.0 ** -7 if device != "cpu" else 1e-5)
+        listed = exact.gather(1, got[2].long())
+        assert float((got[3] - listed).abs().max()) <= off and float((listed - exact.topk(5, dim=1).values).abs().max()) <= 2 * off

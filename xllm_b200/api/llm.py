@@ -391,7 +391,9 @@ class LLM:
 
     def score(self, prompts, top_logprobs: int = 0, temperature: Optional[float] = None) -> List[ScoreOutput]:
         """Log-probability of every token of every prompt under softmax(logits / temperature), with its distribution's entropy and
-        `top_logprobs` alternatives; nothing is generated.  A temperature is 1e-6 to 1e6.  Prompts are strings or token ids; short ones share passes."""
+        `top_logprobs` alternatives; nothing is generated.  A temperature is 1e-6 to 1e6.  Prompts are strings or token ids; short ones share passes.
+        Scores come from fp32 sums, the same with and without alternatives; these and their log-probabilities from the logits that
+        generation samples from, which bf16 rounds (by up to 2^-8 of a logit), so that a token's own score and its entry may differ by that."""
         from .scoring import score_token_lists
         if isinstance(prompts, (str, torch.Tensor)) or (prompts and isinstance(prompts[0], int)):
             prompts = [prompts]

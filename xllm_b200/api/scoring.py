@@ -2,7 +2,8 @@
 
 Prompts are packed into ragged passes on a scratch cache, like embedding requests never in the serving pool.  The tables of a
 pass are built on the device from the prompts' lengths (ops/tables.py); its final hidden states are scored without ever holding
-the logits (ops.score.head_logprobs), or in portions of rows where alternatives are asked for.
+the logits (ops.score.head_logprobs).  Alternatives, where asked for, come from logits in portions of rows, rounded like those that
+tokens are sampled from; the scores are the same with and without them.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ class TokenScores(NamedTuple):
     """Of one prompt, an entry per token; those of the first token are None: nothing comes before it."""
     logprobs: List[Optional[float]]
     entropies: List[Optional[float]]                    # of the distribution that the token was picked from, in nats
-    top_logprobs: Optional[List[Optional[List[tuple]]]]  # [(token id, logprob), ...] most likely first
+    top_logprobs: Optional[List[Optional[List[tuple]]]]  # [(token id, logprob), ...] most likely first; of logits as they are sampled from
 
 
 def _scratch_cache(engine, n_blocks):
@@ -71,13 +72,15 @@ def _score_rows(model, hidden, targets, n_top, temperature):
     head = model.lm_head
     weight = head.weight[:head.vocab]
     t = None if temperature is None else torch.full((hidden.shape[0],), temperature, dtype=torch.float32, device=hidden.device)
-    fused = n_top == 0 and score.head_supported(hidden, weight)
-    parts, step = [], HEAD_ROWS if fused else LOGIT_ROWS
-    for at in range(0, hidden.shape[0], step):
-        h, ids, T = hidden[at:at + step], targets[at:at + step], None if t is None else t[at:at + step]
-        parts.append((*score.head_logprobs(h, weight, ids, temperature=T), None, None) if fused else
-                     score.token_logprobs(model.logits(h), ids, n_top, temperature=T))
-    return [None if p[0] is None else torch.cat(p) for p in zip(*parts)], fused
+    fused = score.head_supported(hidden, weight)
+
+    def portions(rows):
+        return [(hidden[at:at + rows], targets[at:at + rows], None if t is None else t[at:at + rows]) for at in range(0, hidden.shape[0], rows)]
+    from_head = [score.head_logprobs(h, weight, ids, temperature=T) for h, ids, T in portions(HEAD_ROWS)] if fused else []
+    from_logits = [score.token_logprobs(model.logits(h), ids, n_top, temperature=T) for h, ids, T in portions(LOGIT_ROWS)] \
+        if n_top or not fused else []
+    scores = [torch.cat(p) for p in list(zip(*(from_head or from_logits)))[:2]]
+    return scores + ([torch.cat(p) for p in list(zip(*from_logits))[2:]] if n_top else [None, None]), fused
 
 
 @torch.no_grad()

@@ -751,7 +751,8 @@ class ApiServer:
                                  "usage": {"prompt_tokens": len(ids), "total_tokens": len(ids)}})
 
     def _score(self, req, body):
-        """Log-probabilities of the prompts' own tokens: `prompt` (text, token ids, or a list of either), `logprobs` alternatives."""
+        """Log-probabilities of the prompts' own tokens: `prompt` (text, token ids, or a list of either), `logprobs` alternatives, whose
+        log-probabilities are those of rounded logits (`LLM.score`)."""
         from .scoring import score_token_lists
         prompts = body.get("prompt")
         if isinstance(prompts, str) or (isinstance(prompts, list) and prompts and isinstance(prompts[0], int)):
