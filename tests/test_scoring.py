@@ -267,3 +267,40 @@ def test_alternatives_change_no_score(device):
         off = float(logits.abs().max()) / (temperature or 1.0) * (2.0 ** -7 if device != "cpu" else 1e-5)
         listed = exact.gather(1, got[2].long())
         assert float((got[3] - listed).abs().max()) <= off and float((listed - exact.topk(5, dim=1).values).abs().max()) <= 2 * off
+
+
+def test_generation_goes_on_between_passes(tmp_path, monkeypatch):
+    """A request of many passes shares the loop with the requests that generate: a step of theirs behind every pass."""
+    from test_server_cpu import _tokenizer
+    from xllm_b200.api.server import ApiServer
+    eng = engine("cpu", max_tokens_per_batch=32)
+    lists = prompts(20, 25, 70, 1, 30)
+    want = scoring.score_token_lists(eng, lists, 1)
+    srv = ApiServer(eng, _tokenizer(tmp_path), model_name="tiny", host="127.0.0.1", port=0)
+    log, answers = [], []
+    forward, step = scoring._forward, eng.step
+    monkeypatch.setattr(scoring, "_forward", lambda *a: (log.append("pass"), forward(*a))[1])
+    monkeypatch.setattr(eng, "step", lambda *a: (log.append("step"), step(*a))[1])
+    monkeypatch.setattr(srv, "_json", lambda http_id, status, obj: answers.append((http_id, status, obj)))
+    try:
+        eng.add_request("r", prompts(5)[0], max_tokens=40, ignore_eos=True)
+        srv._score(SimpleNamespace(id=1), {"prompt": lists, "logprobs": 1})
+        srv._score(SimpleNamespace(id=2), {"prompt": lists[2]})
+        rounds = 0
+        while srv._busy():
+            srv._after_poll()
+            rounds += 1
+            assert rounds < 200
+        assert log.count("pass") == 6 + 3 and ("pass", "pass") not in zip(log, log[1:]), log
+        assert [(i, status) for i, status, _ in answers] == [(1, 200), (2, 200)]
+        for c, s in zip(answers[0][2]["choices"], want):
+            assert c["logprobs"]["token_logprobs"] == s.logprobs and c["logprobs"]["entropies"] == s.entropies
+        # between two passes the engine may go to sleep: the request ends with an error, the loop goes on
+        srv._score(SimpleNamespace(id=3), {"prompt": lists})
+        srv._after_poll()
+        eng.sleep(1)
+        srv._after_poll()
+        assert not srv._busy() and answers[-1][:2] == (3, 500) and "asleep" in json.dumps(answers[-1][2])
+    finally:
+        srv.shutdown()
+        srv.http.stop()

@@ -83,10 +83,18 @@ def _score_rows(model, hidden, targets, n_top, temperature):
     return scores + ([torch.cat(p) for p in list(zip(*from_logits))[2:]] if n_top else [None, None]), fused
 
 
-@torch.no_grad()
 def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperature: Optional[float] = None) -> List[TokenScores]:
     """Scores of every token of every prompt (token ids), with `n_top` alternatives each, under softmax(logits / temperature).
     RuntimeError where a wait of a kernel expired: its scores are not there."""
+    out, passes = score_in_passes(engine, prompts, n_top, temperature)
+    for _ in passes:
+        pass
+    return out
+
+
+def score_in_passes(engine, prompts, n_top=0, temperature=None):
+    """(scores, passes) of `score_token_lists`: what is asked for is checked here; the scores are filled in while `passes` is gone
+    through, a pass of the model each, between which the engine may step."""
     model, vocab = engine.model, engine.model.lm_head.vocab
     if engine.asleep:
         raise RuntimeError("the engine is asleep")
@@ -103,8 +111,13 @@ def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperat
             raise ValueError(f"a prompt of {len(p)} tokens, the model takes {engine.max_model_len}")
         if any(not 0 <= t < vocab for t in p):
             raise ValueError(f"token ids are 0 to {vocab - 1}")
-    page, dev = engine.cfg.block_size, engine.device
     out = [TokenScores([None] * min(len(p), 1), [None] * min(len(p), 1), [None] * min(len(p), 1) if n_top else None) for p in prompts]
+    return out, _run_passes(engine, prompts, n_top, temperature, out)
+
+
+@torch.no_grad()
+def _run_passes(engine, prompts, n_top, temperature, out):
+    model, page, dev = engine.model, engine.cfg.block_size, engine.device
     whole = bool(getattr(model, "needs_state", False))
     for group in _passes([len(p) for p in prompts], engine.cfg.max_tokens_per_batch, whole):
         longest = max(at + n for work in group for _, at, n in work)
@@ -113,6 +126,8 @@ def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperat
         free = torch.arange(blocks, dtype=torch.int32, device=dev)
         table = torch.zeros(len(group[0]), -(-longest // page), dtype=torch.int32, device=dev)
         for work in group:
+            if engine.asleep:
+                raise RuntimeError("the engine is asleep")
             taken = -(-work[0][1] // page)              # blocks of the passes before; 0 where the pass holds several prompts
             hidden = _forward(engine, prompts, work, table, free[taken:], cache)
             given = [t for i, at, n in work for t in (prompts[i] + [-1])[at + 1:at + n + 1]]
@@ -129,4 +144,4 @@ def score_token_lists(engine, prompts: List[List[int]], n_top: int = 0, temperat
                     out[i].top_logprobs.extend([[(t, v) for t, v in zip(a, b) if t >= 0]
                                                 for a, b in zip(top[row:row + m], top_lps[row:row + m])])
                 row += n
-    return out
+            yield

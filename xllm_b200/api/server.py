@@ -27,6 +27,7 @@ import os
 import queue
 import time
 import uuid
+from collections import deque
 from concurrent.futures import ThreadPoolExecutor
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional
@@ -100,6 +101,7 @@ class ApiServer:
         self.tool_kind = tool_call_parser
         self.reason_kind = reasoning_parser
         self.calls: Dict[str, _Call] = {}
+        self._scoring = deque()     # /v1/score requests under way: (request, body, token ids, scores, passes)
         self.healthy = True
         self.unhealthy_reason = ""
         self.profiler = None
@@ -159,7 +161,7 @@ class ApiServer:
             self._ready.put(None)          # one marker per prepared request (this server counts them)
 
     def _busy(self) -> bool:
-        return (self.engine.has_unfinished() or self._preparing > 0 or
+        return (self.engine.has_unfinished() or self._preparing > 0 or bool(self._scoring) or
                 (self.pd_prefill is not None and self.pd_prefill.has_unfinished()) or
                 any(f._busy() for f in self.forks.values()))
 
@@ -222,6 +224,7 @@ class ApiServer:
                 self.pd_decode = None          # the peer said bye or went away: plain instance again
         elif self.engine.has_unfinished():
             self._dispatch(self.engine.step())
+        self._score_pass()
         self._collect_done()
         self.metrics.tick(len(self.calls))
 
@@ -753,7 +756,7 @@ class ApiServer:
     def _score(self, req, body):
         """Log-probabilities of the prompts' own tokens: `prompt` (text, token ids, or a list of either), `logprobs` alternatives, whose
         log-probabilities are those of rounded logits (`LLM.score`)."""
-        from .scoring import score_token_lists
+        from .scoring import score_in_passes
         prompts = body.get("prompt")
         if isinstance(prompts, str) or (isinstance(prompts, list) and prompts and isinstance(prompts[0], int)):
             prompts = [prompts]
@@ -764,9 +767,27 @@ class ApiServer:
         try:
             ids = [self.tok.encode(p) if isinstance(p, str) else p for p in prompts]
             n_top, t = int(body.get("logprobs") or 0), body.get("temperature")
-            scores = score_token_lists(self.engine, ids, n_top, None if t is None else float(t))
+            scores, passes = score_in_passes(self.engine, ids, n_top, None if t is None else float(t))
         except (TypeError, ValueError) as e:
             return self._error(req.id, 400, str(e))
+        self._scoring.append((req, body, ids, scores, passes))
+
+    def _score_pass(self):
+        """One pass of the oldest scoring request; its answer behind the last one."""
+        if not self._scoring:
+            return
+        req, body, ids, scores, passes = self._scoring[0]
+        try:
+            if next(passes, self._scoring) is not self._scoring:
+                return
+            self._scoring.popleft()
+            self._score_answer(req, body, ids, scores)
+        except Exception as e:
+            if self._scoring and self._scoring[0][0] is req:
+                self._scoring.popleft()
+            self._error(req.id, 500, f"{type(e).__name__}: {e}", "internal_error")
+
+    def _score_answer(self, req, body, ids, scores):
         choices = [{"index": k, "logprobs": {"tokens": [self.tok.decode([t]) for t in i], "token_ids": i, "token_logprobs": s.logprobs,
                                              "entropies": s.entropies,
                                              "top_logprobs": None if s.top_logprobs is None else
