@@ -304,3 +304,20 @@ def test_generation_goes_on_between_passes(tmp_path, monkeypatch):
     finally:
         srv.shutdown()
         srv.http.stop()
+
+
+@pytest.mark.parametrize("number", ["1e999", "-1e999", "NaN"])
+@pytest.mark.parametrize("name", ["logprobs", "temperature"])
+def test_numbers_without_an_integer(tmp_path, monkeypatch, name, number):
+    """What JSON may hold and no 64 bits do is the caller's mistake, not the server's."""
+    from test_server_cpu import _tokenizer
+    from xllm_b200.api.server import ApiServer
+    srv = ApiServer(engine("cpu"), _tokenizer(tmp_path), model_name="tiny", host="127.0.0.1", port=0)
+    answers = []
+    monkeypatch.setattr(srv, "_json", lambda http_id, status, obj: answers.append(status))
+    try:
+        srv._score(SimpleNamespace(id=1), {"prompt": [5, 6], **json.loads('{"%s": %s}' % (name, number))})
+        assert answers == [400]
+    finally:
+        srv.shutdown()
+        srv.http.stop()

@@ -768,7 +768,7 @@ class ApiServer:
             ids = [self.tok.encode(p) if isinstance(p, str) else p for p in prompts]
             n_top, t = int(body.get("logprobs") or 0), body.get("temperature")
             scores, passes = score_in_passes(self.engine, ids, n_top, None if t is None else float(t))
-        except (TypeError, ValueError) as e:
+        except (TypeError, ValueError, OverflowError) as e:
             return self._error(req.id, 400, str(e))
         self._scoring.append((req, body, ids, scores, passes))
 
