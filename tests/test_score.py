@@ -585,3 +585,29 @@ def test_head_uneven_sums(device, kind, T, K, V):
     for a, b, name in zip(got, want, ("logprob", "entropy")):
         off = float((a.double().cpu() - b).norm())
         assert off <= cut + 8 * STEP * float(torch.stack(want).abs().amax(0).norm()), (name, off, cut, float(b.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,V", [(1, 1024, 70000), (1, 2056, 40000), (8, 1032, 9000), (63, 1040, 66000), (64, 1104, 65000), (65, 1104, 65000),
+                                   (100, 704, 100000), (127, 2880, 30000), (128, 512, 20011), (128, 1000, 70000), (128, 4104, 17000),
+                                   (129, 1032, 5003), (130, 1792, 3000), (256, 1800, 4111), (257, 904, 6000), (1000, 2048, 3333),
+                                   (4097, 128, 12345), (4100, 1088, 2051)])
+def test_head_every_row(T, K, V):
+    """Every row, around the numbers of rows and products where the kernel takes another form.  A score is off by what at most 64 steps
+    of the tensor cores cut off, less than 2^-23 of the sum of its products' sizes each, and by a rounding for every chunk of 896 products
+    that is added; a log-probability moves by at most twice as much and has the roundings of `compare`."""
+    h, w, ids, t = head_case(T, K, V, 23, "cuda")
+    ids[::5] = -1
+    for temperature in (None, t):
+        T0 = torch.ones(T, device="cuda").double() if temperature is None else temperature.double()
+        u = h.double() @ w.double().T / T0[:, None]
+        size = (h.double().abs() @ w.double().abs().T).amax(1) / T0
+        lp = torch.log_softmax(u, dim=1)
+        off = 2 * size * (min(K / 16, 64) * 2.0 ** -23 + (K / 896 + 1) * STEP)
+        unit = STEP * (V / 128 + 64)
+        got = score.head_logprobs(h, w, ids, temperature=temperature)
+        asked = lp.gather(1, ids.clamp(min=0)[:, None])[:, 0]
+        far = torch.where(ids < 0, 0.0, (u.amax(1) - u.gather(1, ids.clamp(min=0)[:, None])[:, 0]))
+        near(got[0], torch.where(ids < 0, 0.0, asked).cpu(), (off + unit * (1 + far + math.log(V))).cpu(), "logprob")
+        near(got[1], -(lp.exp() * lp).sum(1).cpu(), ((off + 2 * unit) * (1 + math.log(V))).cpu(), "entropy")
+    assert score.error_status() == 0
