@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   if (row >= p.T) return;                            // whole warps; no block is left by some of the threads of a row
   const float scale = row_scale(p.temperature, row), c = scale * kLog2e;
   const int64_t id = p.ids[row];
-  const bool given = id >= 0 && id < p.V;
+  const bool given = id >= 0 && id < p.V, lost = *p.lost != 0;
+  const float x = given ? p.given[row] : 0.f;        // on its way while the tallies are joined
   const float4* tallies = p.tallies + row * p.n_tiles;
   Tally a = tally_empty();
   for (int i = t; i < p.n_tiles; i += 4 * threads) {
@@ -444,8 +445,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadParams p, int 
   }
   if (t != 0) return;
   // a given token's score is one of those that the tally is made of: no more than its maximum, so that no log-probability is above 0
-  const float lp = given ? tally_logprob(a, p.given[row], scale) : id < 0 ? 0.f : -INFINITY;
-  const bool lost = *p.lost != 0;
+  const float lp = given ? tally_logprob(a, x, scale) : id < 0 ? 0.f : -INFINITY;
   out_lp[row] = lost ? NAN : lp;
   out_entropy[row] = lost ? NAN : tally_entropy(a);
 }
