@@ -8,26 +8,27 @@
 // Many rows: a tile is a pair of CTAs' (cta_group::2), each loads its 128 rows of h and half of the columns' rows of W by TMA into
 // a ring of stages, one thread of the pair's first CTA issues the products into one of two accumulators in tensor memory, and eight
 // warps of each CTA read the other one back, two threads a row, 32 columns at a time.  Bound by the tensor cores; the tally (some
-// 3000 cycles a tile) hides behind the next tile's products where K is 512 and more.
+// 4500 cycles a tile) hides behind the next tile's products where K is 512 and more.
 // Up to 128 rows: a tile is one CTA's and bound by W's way from HBM, and for long by the power that memory and products draw together:
-// up to 64 rows are multiplied by instructions of 64 (45 x 2048 x 151936, sustained: 103 us, 106 with 128; 1 x 4096: 194 us and 199).  An SM's share of the bandwidth depends on its die (of two
-// equal shares one was read in 176 us, the other in 203), so a CTA that is done takes over one that has not started.
+// up to 64 rows are multiplied by instructions of 64 (for seconds 3 % quicker than by those of 128, 45 x 2048 x 151936 and 1 x 4096).  An
+// SM's share of the bandwidth depends on its die (of two equal shares one was read in 176 us, the other in 203), so a CTA that is done
+// takes over one that has not started.
 //
-//   one B200             floor   time        (us; 6536 GB/s, 1670 TFLOP/s)
-//   1 x 4096 x 151936      190    192        6.5 TB/s
-//   45 x 2048 x 151936      95    100
-//   128 x 4096 x 151936    191    199
-//   200 x 4096 x 151936    191    240        power, of memory and products of 256 rows; takeover by pairs 250, 256 rows on a single CTA 257
-//   1000 x 4096 x 32768    161    181
-//   4096 x 512 x 151936    382    449        the tally
-//   4096 x 4096 x 151936  3053   3080        0.99 of the burst rate
+//   one B200             floor   time  for seconds        (us, back to back from a graph; 6536 GB/s, 1670 TFLOP/s)
+//   1 x 4096 x 151936      190    192    194    6.5 TB/s
+//   45 x 2048 x 151936      95    100    106
+//   128 x 4096 x 151936    191    202    227    power, of memory and products
+//   200 x 4096 x 151936    191    252    313    the same, of products of 256 rows; 10 more with takeover by pairs, 15 with 256 rows on a single CTA
+//   1000 x 4096 x 32768    161    180    213
+//   4096 x 512 x 151936    382    450           the tally
+//   4096 x 4096 x 151936  3053   3060   3520    the burst rate; for seconds above the sustained one (3626)
 //
 // The tensor cores cut a sum of products off at each of its K / 16 steps, by 2^-26 of what is there on average (measured against 64 bits:
 // scores of dense rows come out smaller by 0.94e-9 K of themselves, those of one large channel in front of all others by twice that).  So
 // no more than 1024 products are summed there: longer rows in chunks of up to 896, whose sums are added up in fp32, with rounding, by the
 // threads that read the accumulators.  Off against 64 bits, relative, 1000 x 4096 x 32768: log-probabilities 3.2e-7, entropies 2.0e-7 (a
-// product in fp32 3.5e-7 and 1.4e-7; unchunked 1.5e-6).  For seconds, unchunked and in chunks: 4096 x 4096 x 151936 3636 and 3663 us, in
-// chunks of 512 3823; 4096 x 1536 x 151936 1386 and 1417; 45 x 2048 x 151936 105 and 106.
+// product in fp32 3.5e-7 and 1.4e-7; unchunked 1.5e-6).  Chunks cost time where power is short: 4096 x 1536 x
+// 151936 for seconds 1388 us, 1358 unchunked; 200 x 4096 x 151936 313 and 308; 4096 x 4096 x 151936 nothing, in chunks of 512 4 %.
 //
 // Every wait is bounded; on expiry the kernel raises an error word and the call's own, all roles leave their loops, tensor memory is
 // freed and the kernel returns.  What the call's tiles would have been is then not there: all its results are NaN.
