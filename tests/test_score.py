@@ -611,3 +611,33 @@ def test_head_every_row(T, K, V):
         near(got[0], torch.where(ids < 0, 0.0, asked).cpu(), (off + unit * (1 + far + math.log(V))).cpu(), "logprob")
         near(got[1], -(lp.exp() * lp).sum(1).cpu(), ((off + 2 * unit) * (1 + math.log(V))).cpu(), "entropy")
     assert score.error_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,V", [(33, 2056, 9000), (100, 1032, 9000), (300, 2056, 9000)])
+def test_chunked_rows_repeat(T, K, V):
+    """Sums of several chunks have the same bits in every call: beside another call on another stream, and captured, where the replayed
+    graph reads what is in its inputs' places then."""
+    from xllm_b200.ops import gemm_tcgen05
+    gemm_tcgen05.prepare()
+    h, w, ids, t = head_case(T, K, V, 31, "cuda")
+    h2, _, ids2, _ = head_case(T, K, V, 32, "cuda")
+    want, want2 = score.head_logprobs(h, w, ids, temperature=t), score.head_logprobs(h2, w, ids2, temperature=t)
+    torch.cuda.synchronize()
+    got, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(6):
+        for s, a, b in zip(streams, (h, h2), (ids, ids2)):
+            with torch.cuda.stream(s):
+                got.append(score.head_logprobs(a, w, b, temperature=t))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, (want, want2)[i % 2]))
+    g, place, asked = torch.cuda.CUDAGraph(), h.clone(), ids.clone()
+    with torch.cuda.graph(g):
+        out = score.head_logprobs(place, w, asked, temperature=t)
+    for a, b, c in ((h, ids, want), (h2, ids2, want2), (h, ids, want)):
+        place.copy_(a), asked.copy_(b)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, c))
+    assert score.error_status() == 0
